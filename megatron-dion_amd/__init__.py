@@ -29,6 +29,17 @@ from .batches import build_dion_batches  # noqa: F401
 from .runtime import AsyncRuntime, batch_dion_update_async  # noqa: F401
 from .optimizer import MegatronDion  # noqa: F401
 from .grad_norm import dion_grad_norm, dion_grad_norm_sq  # noqa: F401
+from .lm_autograd import dropout_add, linear_cross_entropy, rms_norm_add  # noqa: F401
+from .lm_ops import (  # noqa: F401
+    RmsNormAdd,
+    RmsNormAddGrads,
+    dropout_add_backward,
+    dropout_add_forward,
+    linear_cross_entropy_backward,
+    linear_cross_entropy_forward,
+    rms_norm_add_backward,
+    rms_norm_add_forward,
+)
 
 __all__ = [
     "MegatronDion",
@@ -52,4 +63,15 @@ __all__ = [
     "init_dion_state",
     "dion_grad_norm_sq",
     "dion_grad_norm",
+    "linear_cross_entropy",
+    "rms_norm_add",
+    "dropout_add",
+    "linear_cross_entropy_forward",
+    "linear_cross_entropy_backward",
+    "rms_norm_add_forward",
+    "rms_norm_add_backward",
+    "dropout_add_forward",
+    "dropout_add_backward",
+    "RmsNormAdd",
+    "RmsNormAddGrads",
 ]

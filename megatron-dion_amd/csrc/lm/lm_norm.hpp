@@ -1,0 +1,327 @@
+// lm_norm.hpp -- residual RMS norm with dropout, 8-bit output, and its backward pass.
+//
+// One pass over the data: a row is held in registers (NV vectors of VEC elements for each of the
+// LPR threads that share it) between its sum of squares and its scaling, so the forward reads x
+// and the residual and writes h and y once, and the backward reads gy, h and grad_h and writes the
+// gradients once.  Rows of up to 1024 elements go to a wave each (no barrier), longer ones to a
+// block.  VEC = 8 needs 16-byte aligned rows; VEC = 1 takes everything else.
+
+struct NormArgs {
+  const void *x, *residual, *weight, *gy, *gh;
+  const void* h_in;
+  void *h, *y, *gx, *gr, *gw;
+  float *scale, *rstd_out, *part;
+  const float* rstd;
+  int64_t rows;
+  int cols, w_bf16, gw_bf16, accumulate, sblock, sblocks;
+  float eps;
+  int64_t ldx, ldr, ldh, ldy, ldgy, ldgh, ldgx, ldgr;
+  DropArgs drop;
+  int dropping;
+};
+
+template <int VEC>
+__device__ __forceinline__ void load_weight(const NormArgs& a, int c, float* w) {
+  if (a.w_bf16) load_vec<VEC>(static_cast<const bf16*>(a.weight) + c, w);
+  else load_vec<VEC>(static_cast<const float*>(a.weight) + c, w);
+}
+
+// sum over the LPR threads that share a row; `red`: LPR / 64 floats of LDS (LPR > 64)
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = wave_sum(v);
+  if constexpr (LPR > 64) {
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();  // the last use of red is over
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LPR / 64; ++i) v += red[i];
+  }
+  return v;
+}
+
+__device__ __forceinline__ float e4m3_clamp(float v) {  // NaN stays NaN
+  return v > 448.0f ? 448.0f : v < -448.0f ? -448.0f : v;
+}
+
+// threads of a block: 4 rows of 64 threads, or one row of LPR
+template <int LPR>
+constexpr int norm_threads() { return LPR > 64 ? LPR : 256; }
+
+template <typename T, int VEC, int LPR, int NV, bool QUANT>
+__global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const NormArgs a) {
+  constexpr int RPB = LPR > 64 ? 1 : 4;
+  __shared__ float red[16];
+  extern __shared__ uint32_t amax[];  // QUANT: sblocks words for each row of the block
+  const int t = LPR > 64 ? threadIdx.x : (threadIdx.x & 63);
+  const int sub = LPR > 64 ? 0 : (threadIdx.x >> 6);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + sub;
+  const bool live = row < a.rows;  // whole waves: RPB == 4 has a row for each wave
+  float v[NV][VEC];
+  if constexpr (QUANT) {
+    for (int i = t; i < a.sblocks; i += LPR) amax[sub * a.sblocks + i] = 0u;
+    __syncthreads();
+  }
+  float ss = 0.0f;
+  if (live) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = static_cast<const T*>(a.residual) + row * a.ldr;
+    T* h = static_cast<T*>(a.h) + row * a.ldh;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) load_vec<VEC>(x + c, v[i]);
+    }
+    float q[NV][VEC];
+    if (a.residual) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        if (c < a.cols) load_vec<VEC>(r + c, q[i]);
+      }
+    }
+    if (a.dropping) {
+      const Key key = philox_key(a.drop);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        if (c < a.cols) drop_vec<VEC>(v[i], static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          if (a.residual) v[i][k] = __fadd_rn(v[i][k], q[i][k]);
+          v[i][k] = to_f32(from_f32<T>(v[i][k]));  // the norm is of h as it is stored
+          ss = fmaf(v[i][k], v[i][k], ss);
+        }
+        if (a.h) store_vec<VEC>(h + c, v[i]);
+      }
+    }
+  }
+  ss = row_sum<LPR>(ss, red);
+  const float rstd = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  if (live && t == 0) a.rstd_out[row] = rstd;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) {
+        float w[VEC];
+        load_weight<VEC>(a, c, w);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[i][k] = v[i][k] * rstd * w[k];
+        if constexpr (!QUANT) store_vec<VEC>(static_cast<T*>(a.y) + row * a.ldy + c, v[i]);
+      }
+    }
+  }
+  if constexpr (QUANT) {
+    // |y| as bits is ordered like an integer; a maximum does not depend on the order it is taken in
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        if (c < a.cols) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            const float y = fabsf(v[i][k]);
+            if (y == y) atomicMax(&amax[sub * a.sblocks + (c + k) / a.sblock], __float_as_uint(y));
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (live) {
+      for (int i = t; i < a.sblocks; i += LPR)
+        a.scale[row * a.sblocks + i] = fmaxf(__uint_as_float(amax[sub * a.sblocks + i]) / 448.0f, 1.17549435e-38f);
+      uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        if (c < a.cols) {
+          uint8_t b[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            const float s = fmaxf(__uint_as_float(amax[sub * a.sblocks + (c + k) / a.sblock]) / 448.0f, 1.17549435e-38f);
+            b[k] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[i][k] / s), 0.0f, 0, false) & 0xFF);
+          }
+          for (int k = 0; k < VEC; ++k) y[c + k] = b[k];
+        }
+      }
+    }
+  }
+}
+
+// Weight-gradient partials: each block (or wave, LPR == 64) sums its rows in registers.
+template <typename T, int VEC, int LPR, int NV>
+__global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const NormArgs a) {
+  constexpr int RPB = LPR > 64 ? 1 : 4;
+  __shared__ float red[16];
+  const int t = LPR > 64 ? threadIdx.x : (threadIdx.x & 63);
+  const int64_t first = LPR > 64 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
+  float w[NV][VEC], dw[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LPR + t) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[i][k] = dw[i][k] = 0.0f;
+    if (c < a.cols) load_weight<VEC>(a, c, w[i]);
+  }
+  Key key = {0, 0, 0, 0};
+  if (a.dropping) key = philox_key(a.drop);
+  for (int64_t row = first; row < a.rows; row += step) {
+    const float rstd = a.rstd[row];
+    float u[NV][VEC], g[NV][VEC], dot = 0.0f;  // u = h rstd, g = gy then w gy
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) {
+        load_vec<VEC>(static_cast<const T*>(a.h_in) + row * a.ldh + c, u[i]);
+        load_vec<VEC>(static_cast<const T*>(a.gy) + row * a.ldgy + c, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          u[i][k] *= rstd;
+          dw[i][k] = fmaf(g[i][k], u[i][k], dw[i][k]);
+          g[i][k] *= w[i][k];
+          dot = fmaf(g[i][k], u[i][k], dot);
+        }
+      }
+    }
+    if (a.gx || a.gr) {
+      const float mean = row_sum<LPR>(dot, red) / static_cast<float>(a.cols);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        if (c < a.cols) {
+          float d[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) d[k] = rstd * (g[i][k] - u[i][k] * mean);
+          if (a.gh) {
+            float q[VEC];
+            load_vec<VEC>(static_cast<const T*>(a.gh) + row * a.ldgh + c, q);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) d[k] += q[k];
+          }
+          if (a.gr) store_vec<VEC>(static_cast<T*>(a.gr) + row * a.ldgr + c, d);
+          if (a.gx) {
+            if (a.dropping) drop_vec<VEC>(d, static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
+            store_vec<VEC>(static_cast<T*>(a.gx) + row * a.ldgx + c, d);
+          }
+        }
+      }
+    }
+  }
+  if (a.part) {
+    float* p = a.part + first * a.cols;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LPR + t) * VEC;
+      if (c < a.cols) store_vec<VEC>(p + c, dw[i]);
+    }
+  }
+}
+
+// grad_weight = the sum of the partials in a fixed order: 32 columns a block, 8 threads a column
+__global__ void __launch_bounds__(256) norm_dw_kernel(const NormArgs a, int parts) {
+  __shared__ float red[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (c < a.cols)
+    for (int i = k; i < parts; i += 8) s += a.part[static_cast<int64_t>(i) * a.cols + c];
+  red[k][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (k == 0 && c < a.cols) {
+    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x & 31];
+    if (a.gw_bf16) {
+      uint16_t* o = static_cast<uint16_t*>(a.gw) + c;
+      *o = f32_to_bf16(a.accumulate ? bf16_to_f32(*o) + s : s);
+    } else {
+      float* o = static_cast<float*>(a.gw) + c;
+      *o = a.accumulate ? *o + s : s;
+    }
+  }
+}
+
+namespace rms {
+
+constexpr int kMaxCols = 16384;
+
+// partials of grad_weight: blocks of the backward kernel (two for each CU: every one reads the
+// weight once and leaves one partial row), times the rows that a block works on at once
+long bwd_blocks(int64_t rows, bool wave_rows) {
+  const long want = wave_rows ? ceil_div(rows, 4) : rows;
+  return want < 512 ? (want < 1 ? 1 : want) : 512;
+}
+bool wave_rows(int cols, bool vec) { return vec ? cols <= 1024 : cols <= 512; }
+
+size_t ws_bytes(const DionNormDesc* d) {  // the larger of the two layouts: alignment is not known here
+  const long a = bwd_blocks(d->rows, true) * 4, b = bwd_blocks(d->rows, false);
+  return sizeof(float) * static_cast<size_t>(a > b ? a : b) * d->cols;
+}
+
+template <typename T, bool QUANT>
+int forward(const NormArgs& a, bool vec, hipStream_t st) {
+#define DION_NORM_FWD(VEC, LPR, NV)                                                                            \
+  do {                                                                                                         \
+    constexpr int RPB = LPR > 64 ? 1 : 4;                                                                      \
+    const size_t lds = QUANT ? sizeof(uint32_t) * RPB * a.sblocks : 0;                                         \
+    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, LPR, NV, QUANT>), dim3(ceil_div(a.rows, RPB)),                 \
+                       dim3(norm_threads<LPR>()), lds, st, a);                                                 \
+  } while (0)
+  if (vec) {
+    if (a.cols <= 512) DION_NORM_FWD(8, 64, 1);
+    else if (a.cols <= 1024) DION_NORM_FWD(8, 64, 2);
+    else if (a.cols <= 2048) DION_NORM_FWD(8, 256, 1);
+    else if (a.cols <= 4096) DION_NORM_FWD(8, 256, 2);
+    else if (a.cols <= 8192) DION_NORM_FWD(8, 512, 2);
+    else DION_NORM_FWD(8, 1024, 2);
+  } else {
+    if (a.cols <= 512) DION_NORM_FWD(1, 64, 8);
+    else if (a.cols <= 1024) DION_NORM_FWD(1, 256, 4);
+    else if (a.cols <= 4096) DION_NORM_FWD(1, 256, 16);
+    else DION_NORM_FWD(1, 1024, 16);
+  }
+#undef DION_NORM_FWD
+  return check_launch("rms_norm_add");
+}
+
+template <typename T>
+int backward(const NormArgs& a, bool vec, hipStream_t st) {
+  const bool wr = wave_rows(a.cols, vec);
+  const long blocks = bwd_blocks(a.rows, wr);
+#define DION_NORM_BWD(VEC, LPR, NV)                                                                         \
+  hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, LPR, NV>), dim3(blocks), dim3(norm_threads<LPR>()), 0, st, a)
+  if (vec) {
+    if (a.cols <= 512) DION_NORM_BWD(8, 64, 1);
+    else if (a.cols <= 1024) DION_NORM_BWD(8, 64, 2);
+    else if (a.cols <= 2048) DION_NORM_BWD(8, 256, 1);
+    else if (a.cols <= 4096) DION_NORM_BWD(8, 256, 2);
+    else if (a.cols <= 8192) DION_NORM_BWD(8, 512, 2);
+    else DION_NORM_BWD(8, 1024, 2);
+  } else {
+    if (a.cols <= 512) DION_NORM_BWD(1, 64, 8);
+    else if (a.cols <= 1024) DION_NORM_BWD(1, 256, 4);
+    else if (a.cols <= 4096) DION_NORM_BWD(1, 256, 16);
+    else DION_NORM_BWD(1, 1024, 16);
+  }
+#undef DION_NORM_BWD
+  int rc = check_launch("rms_norm_add_backward");
+  if (rc != DION_OK || a.gw == nullptr) return rc;
+  hipLaunchKernelGGL(norm_dw_kernel, dim3(ceil_div(a.cols, 32)), dim3(256), 0, st, a,
+                     static_cast<int>(blocks * (wr ? 4 : 1)));
+  return check_launch("rms_norm_add_backward(weight)");
+}
+
+}  // namespace rms
