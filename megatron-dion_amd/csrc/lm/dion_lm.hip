@@ -143,9 +143,11 @@ int dion_rms_norm_add(const DionNormDesc* d, const void* x, const void* residual
                    d->ld_y % 8 == 0 &&
                    (!residual || (aligned16(residual) && d->ld_residual % 8 == 0)) &&
                    (!h || (aligned16(h) && d->ld_h % 8 == 0));
-  if (d->dtype == DION_DTYPE_F32)
-    return quant ? rms::forward<float, true>(a, vec, stream) : rms::forward<float, false>(a, vec, stream);
-  return quant ? rms::forward<bf16, true>(a, vec, stream) : rms::forward<bf16, false>(a, vec, stream);
+  const bool f32 = d->dtype == DION_DTYPE_F32;
+  if (!quant) return f32 ? rms::forward<float, Q8_NONE>(a, vec, stream) : rms::forward<bf16, Q8_NONE>(a, vec, stream);
+  const bool lanes = vec && a.sblock >= 8 && a.sblock <= 512 && (a.sblock & (a.sblock - 1)) == 0;
+  if (lanes) return f32 ? rms::forward<float, Q8_LANES>(a, vec, stream) : rms::forward<bf16, Q8_LANES>(a, vec, stream);
+  return f32 ? rms::forward<float, Q8_ANY>(a, vec, stream) : rms::forward<bf16, Q8_ANY>(a, vec, stream);
 }
 
 int dion_rms_norm_add_workspace_bytes(const DionNormDesc* d, size_t* bytes) {

@@ -15,7 +15,7 @@
 // bits each); a product of them is a list of segments, the limb pairs that matter, which the loop
 // walks through as if k were that much longer.  Accumulation is fp32 in the MFMA.
 //
-// Tiles go to LDS by buffer_load_dwordx4 ... lds, NBUF - 1 steps of 64 k ahead; rows and columns
+// Tiles go to LDS by buffer_load_dwordx4 ... lds, NBUF - 1 to NBUF steps of 64 k ahead; rows and columns
 // past the end get an offset past the descriptor's range, which loads zeros.  16-byte chunks are
 // placed so that the reads of a wave spread over all banks: KC chunk c of row r at c ^ (r/2 % 8),
 // KS 64-byte slot s of row k at s ^ (k%4 + 4 (k/8 % 2)).
@@ -44,7 +44,7 @@ struct GemmArgs {
   const float* lse;      // per compact token
   const float* gl;       // per compact token: upstream gradient
   int col0;              // first shard column of this piece
-  float2* part;          // stats: [part][token] (max, sum)
+  float2* part;          // stats: [part][token] (c, sum of 2^(x log2(e) - c))
   float* tlogit;         // stats: per compact token
   int64_t ldpart;
   uint16_t* g[3];        // limbs of g
@@ -68,41 +68,41 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // (wait_barrier), which is why this is asm and not the builtin: with the builtin hipcc waits for
 // all of them before any LDS read.
 __device__ __forceinline__ void load_lds16(const i32x4& rsrc, uint32_t voff, uint32_t lds) {
-  unsigned keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-      : "=&s"(keep)
-      : "v"(voff), "s"(rsrc), "s"(lds)
-      : "memory");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
-__device__ __forceinline__ i32x4 make_rsrc(const void* p) {
+__device__ __forceinline__ i32x4 make_rsrc(const void* p, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(p);
   i32x4 r;
   r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(a));
   r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>((a >> 32) & 0xFFFF));
-  r[2] = static_cast<int>(kOob);
+  r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
   r[3] = 0x00020000;
   return r;
 }
 
-// One operand's tile: BN rows (KC) or columns (KS) by 64 k, loaded by NW waves.
-template <int BN, bool KS, int NW>
+// One operand's tile: BN rows (KC) or columns (KS) by 64 k, loaded by NW waves in units of 1 KiB.
+// KTAIL: the operand ends with k in memory; the other operand is zero there, but 0 x NaN is not.
+template <int BN, bool KS, int NW, bool KTAIL>
 struct Tile {
   static constexpr int kBytes = BN * kBK * 2;
-  static constexpr int kUnits = kBytes / 1024;  // wave loads
+  static constexpr int kUnits = kBytes / 1024;
   static constexpr int kPerWave = kUnits / NW;
   static constexpr int kRowBytes = KS ? BN * 2 : 128;
   static constexpr int kUnitRows = 1024 / kRowBytes;
   static_assert(kUnits % NW == 0, "every wave issues the same number of loads");
   uint32_t voff[kPerWave];
-  int kk[kPerWave];  // k of the lane's chunk within the tile
+  int kk[kPerWave];  // KC with KTAIL: k of the lane's chunk within the tile
+  uint32_t ldb;      // bytes of a row in memory
+  i32x4 rsrc;
+  int kleft;
 
   // first: first row (KC) / column (KS) of the tile; limit: rows / columns that exist
   __device__ __forceinline__ void init(int wave, int lane, int first, int limit, int64_t ld) {
+    ldb = static_cast<uint32_t>(ld * 2);
 #pragma unroll
     for (int u = 0; u < kPerWave; ++u) {
       const int unit = wave * kPerWave + u;
@@ -112,24 +112,26 @@ struct Tile {
       if constexpr (KS) {
         const int f = ((row & 3) | (((row >> 3) & 1) << 2)) & (BN / 32 - 1);
         const int chunk = pos ^ (f << 2);
-        kk[u] = row;
-        voff[u] = first + chunk * 8 < limit ? static_cast<uint32_t>(row * ld * 2 + chunk * 16) : kOob;
+        voff[u] = first + chunk * 8 < limit ? row * ldb + chunk * 16 : kOob;
       } else {
         const int chunk = pos ^ ((row >> 1) & 7);
         kk[u] = chunk * 8;
-        voff[u] = first + row < limit ? static_cast<uint32_t>(row * ld * 2 + chunk * 16) : kOob;
+        voff[u] = first + row < limit ? row * ldb + chunk * 16 : kOob;
       }
     }
   }
-  // kleft: k that exist from this step on
-  __device__ __forceinline__ void issue(const void* base, int wave, uint32_t lds, int kleft) const {
-    const i32x4 rsrc = make_rsrc(base);
-#pragma unroll
-    for (int u = 0; u < kPerWave; ++u) {
-      uint32_t v = voff[u];
-      if (kleft < kBK) v = kk[u] < kleft ? v : kOob;
-      load_lds16(rsrc, v, lds + (wave * kPerWave + u) * 1024);
-    }
+  // A step: base is the tile's first byte there; k_left: k that exist from it on (0: past the end,
+  // everything loads zeros).  A KS tile ends with its descriptor's range, a KC tile lane by lane.
+  __device__ __forceinline__ void step(const void* base, int k_left) {
+    kleft = k_left;
+    const uint32_t range = KS && k_left < kBK ? k_left * ldb : k_left > 0 ? kOob : 0u;
+    rsrc = make_rsrc(base, range);
+  }
+  template <int U>
+  __device__ __forceinline__ void issue(int wave, uint32_t lds) const {
+    uint32_t v = voff[U];
+    if constexpr (!KS && KTAIL) v = kk[U] < kleft ? v : kOob;
+    load_lds16(rsrc, v, lds + (wave * kPerWave + U) * 1024);
   }
 };
 
@@ -170,26 +172,41 @@ struct Frag {
 };
 
 // Tiles in an order that lets the blocks that run together share operands: blocks go round-robin
-// to the 8 XCDs, so each XCD gets a contiguous range of tiles, walked in columns of 8 row tiles.
+// to the 8 XCDs, so each XCD gets a contiguous range of tiles, walked in columns of 4 row tiles (measured
+// on 32 x 501 tiles of 256 x 256: 1241 TFLOP/s against 1224 in columns of 8 and 1174 of 16).
 __device__ __forceinline__ void tile_of(int id, int row_tiles, int col_tiles, int* rt, int* ct) {
   const int n = row_tiles * col_tiles, xcd = id & 7, local = id >> 3;
   const int per = n >> 3, extra = n & 7;
   const int t = xcd * per + (xcd < extra ? xcd : extra) + local;
-  const int group = 8 * col_tiles, g = t / group, r0 = g * 8;
-  const int gr = row_tiles - r0 < 8 ? row_tiles - r0 : 8;
+  const int group = 4 * col_tiles, g = t / group, r0 = g * 4;
+  const int gr = row_tiles - r0 < 4 ? row_tiles - r0 : 4;
   const int in = t - g * group;
   *rt = r0 + in % gr;
   *ct = in / gr;
 }
 
-constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
+// compile-time loop: f(integral_constant 0), ..., f(N - 1)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
+
+// The loop over steps of 64 k is software-pipelined by hand.  A step is four phases of 16 k; in each,
+// a wave's MFMAs run on fragments in registers while it reads the next phase's from LDS.  The barrier
+// stands before the last phase: there every wave has its last fragments of this step's tile, so the
+// tile's buffer is free for the step NBUF on, whose loads are issued in between the phase's MFMAs, and
+// the next step's tile has arrived (vmcnt), whose first fragments the phase reads.
 template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, int EPI, int NBUF>
 __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const GemmArgs a) {
   constexpr int NWR = BR / WR, NWC = BC / WC, NW = NWR * NWC;
   constexpr int TR = WR / 32, TC = WC / 32;
-  using RT = Tile<BR, RKS, NW>;
-  using CT = Tile<BC, CKS, NW>;
+  using RT = Tile<BR, RKS, NW, false>;
+  using CT = Tile<BC, CKS, NW, true>;
   constexpr int kStage = RT::kBytes + CT::kBytes;
   constexpr int kLoads = RT::kPerWave + CT::kPerWave;
   extern __shared__ __align__(16) char lds[];
@@ -225,161 +242,233 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
+  static_assert(NW * 32 * WC * 4 <= NBUF * kStage, "the epilogue's rows fit");
   const uint32_t lds0 = lds_addr(lds);
-  int seg = 0, ks_at = k_lo;
-  auto issue = [&](int step) {
-    const uint32_t at = lds0 + static_cast<uint32_t>(step % NBUF) * kStage;
-    const bool real = step < steps;  // past the end: zeros, so that the counts of the waits hold
-    const int64_t k0 = static_cast<int64_t>(ks_at) * kBK;
-    const uint16_t* rp = a.r[seg] + (RKS ? k0 * a.ldr + row0 : static_cast<int64_t>(row0) * a.ldr + k0);
-    const uint16_t* cp = a.c[seg] + (CKS ? k0 * a.ldc + c0 : static_cast<int64_t>(c0) * a.ldc + k0);
-    rtile.issue(rp, wave, at, real ? kBK : 0);
-    ctile.issue(cp, wave, at + RT::kBytes, real ? k_all - static_cast<int>(k0) : 0);
-    if (real && ++ks_at == k_hi && seg + 1 < a.nseg) {
-      ks_at = k_lo;
-      ++seg;
+  // The next step's addresses, kept in scalar registers and made while MFMAs run; past the end a step
+  // loads zeros, so that the counts of the waits hold.
+  const int64_t rstep = RKS ? a.ldr * (2 * kBK) : 2 * kBK, cstep = CKS ? a.ldc * (2 * kBK) : 2 * kBK;
+  const int64_t rfirst = RKS ? k_lo * rstep + row0 * 2 : row0 * a.ldr * 2 + k_lo * rstep;
+  const int64_t cfirst = CKS ? k_lo * cstep + c0 * 2 : c0 * a.ldc * 2 + k_lo * cstep;
+  const char* rp = reinterpret_cast<const char*>(a.r[0]) + rfirst;
+  const char* cp = reinterpret_cast<const char*>(a.c[0]) + cfirst;
+  int seg = 0, left = per_seg, k_left = k_all - k_lo * kBK;  // steps and k of this segment
+  uint32_t slot = 0, into = lds0;
+  auto next_step = [&]() {
+    rtile.step(rp, left > 0 ? kBK : 0);
+    ctile.step(cp, left > 0 ? k_left : 0);
+    into = lds0 + slot;
+    slot = slot + kStage == NBUF * kStage ? 0 : slot + kStage;
+    rp += rstep;
+    cp += cstep;
+    k_left -= kBK;
+    if (--left == 0 && ++seg < a.nseg) {
+      rp = reinterpret_cast<const char*>(a.r[seg]) + rfirst;
+      cp = reinterpret_cast<const char*>(a.c[seg]) + cfirst;
+      left = per_seg;
+      k_left = k_all - k_lo * kBK;
     }
   };
+  auto issue = [&](auto u) {
+    constexpr int U = decltype(u)::value;
+    if constexpr (U < RT::kPerWave) rtile.template issue<U>(wave, into);
+    else ctile.template issue<U - RT::kPerWave>(wave, into + RT::kBytes);
+  };
+  bf16x8 cv[2][TC], rv[2][TR];
+  auto read = [&](int set, auto q, const char* stage, int ks) {
+    constexpr int Q = decltype(q)::value;
+    if constexpr (Q < TC) cv[set][Q] = cf.read(stage + RT::kBytes, wc * TC + Q, ks);
+    else rv[set][Q - TC] = rf.read(stage, wr * TR + Q - TC, ks);
+  };
   if (steps > 0) {
-#pragma unroll
-    for (int s = 0; s < NBUF - 1; ++s) issue(s);
+    each<NBUF>([&](auto) {
+      next_step();
+      each<kLoads>(issue);
+    });
+    wait_barrier<kLoads*(NBUF - 1)>();
+    each<TC + TR>([&](auto q) { read(0, q, lds, 0); });
   }
+  uint32_t at = 0;
   for (int step = 0; step < steps; ++step) {
-    wait_barrier<kLoads*(NBUF - 2)>();  // this step's tile is there; all have read the one before
-    issue(step + NBUF - 1);
-    const char* rb = lds + (step % NBUF) * kStage;
-    const char* cb = rb + RT::kBytes;
+    const char* now = lds + at;
+    at = at + kStage == NBUF * kStage ? 0 : at + kStage;
+    const char* then = lds + at;
+    each<4>([&](auto phase) {
+      constexpr int P = decltype(phase)::value, set = P & 1;
+      if constexpr (P == 1) next_step();
+      if constexpr (P == 3) wait_barrier<kLoads*(NBUF - 2)>();
+      __builtin_amdgcn_sched_barrier(0);
+      each<TC * TR>([&](auto m) {
+        constexpr int M = decltype(m)::value, i = M / TR, j = M % TR;
+        constexpr int NM = TC * TR, NR = TC + TR;
+        constexpr int per = (NR + NM - 1) / NM;  // reads after each MFMA until there are none left
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cv[set][i], rv[set][j], acc[i][j], 0, 0, 0);
+        each<per>([&](auto r) {
+          constexpr int Q = M * per + decltype(r)::value;
+          if constexpr (Q < NR) read(set ^ 1, std::integral_constant<int, Q>{}, P == 3 ? then : now, (P + 1) & 3);
+        });
+        if constexpr (P == 3) {
+          constexpr int lo = M * kLoads / NM, hi = (M + 1) * kLoads / NM;
+          each<hi - lo>([&](auto u) { issue(std::integral_constant<int, lo + decltype(u)::value>{}); });
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+  }
+  // no load into LDS outlives the loop, and no wave still reads a tile: the epilogue takes the memory
+  wait_barrier<0>();
+
+  // lane: row row0 + wr WR + 32 j + lane % 32, columns cw + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
+  const int hi = lane >> 5, hi4 = hi * 4;
+  const int cw = c0 + wc * WC;
+  const bool whole = c0 + BC <= a.cols;  // no column of the tile is past the end
+  if constexpr (EPI == EPI_STATS) {
+    // Exponentials to base 2: x log2(e) - c is one fma, and c (the rounded maximum) one exact number in
+    // both the terms and the result, so that its rounding does not matter.
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      bf16x8 cv[TC], rv[TR];
+    for (int j = 0; j < TR; ++j) {
+      const int row = row0 + wr * WR + 32 * j + (lane & 31);
+      const int tgt = row < n_valid ? a.tgt[row] - a.col0 - cw : -1;  // column within the wave's
+      if (!whole) {
 #pragma unroll
-      for (int i = 0; i < TC; ++i) cv[i] = cf.read(cb, wc * TC + i, ks);
+        for (int i = 0; i < TC; ++i)
 #pragma unroll
-      for (int j = 0; j < TR; ++j) rv[j] = rf.read(rb, wr * TR + j, ks);
+          for (int e = 0; e < 16; ++e)
+            if (cw + 32 * i + 8 * (e >> 2) + hi4 + (e & 3) >= a.cols) acc[i][j][e] = -INFINITY;
+      }
+      if (__any(tgt >= 0 && tgt < WC)) {
+#pragma unroll
+        for (int i = 0; i < TC; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * i + 8 * (e >> 2) + hi4 + (e & 3) == tgt) a.tlogit[row] = acc[i][j][e];
+      }
+      float m = acc[0][j][0];
 #pragma unroll
       for (int i = 0; i < TC; ++i)
 #pragma unroll
-        for (int j = 0; j < TR; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cv[i], rv[j], acc[i][j], 0, 0, 0);
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float c = m == -INFINITY ? 0.0f : m * kLog2e;
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < TC; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e & 3] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], kLog2e, -c));
+      float sum = (s[0] + s[1]) + (s[2] + s[3]);
+      sum += __shfl_xor(sum, 32, 64);
+      if (lane < 32 && row < n_valid)
+        a.part[(static_cast<int64_t>(a.col0 / BC + ct) * NWC + wc) * a.ldpart + row] =
+            make_float2(m == -INFINITY ? m : c, sum);
     }
+    return;
   }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no load into LDS outlives the loop
-
-  // lane: row row0 + wr WR + 32 j + lane % 32, columns c0 + wc WC + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4
-  const int hi4 = (lane >> 5) * 4;
-  const int cw = c0 + wc * WC;
+  // The others store matrices: 32 rows at a time go through the wave's own LDS, so that a store
+  // instruction writes whole cache lines.  Chunk c (4 columns) of row r lies at c ^ r.
+  constexpr int CH = WC / 4, kRowsAt = 64 / CH;
+  float* mine = reinterpret_cast<float*>(lds) + wave * (32 * WC);
 #pragma unroll
   for (int j = 0; j < TR; ++j) {
-    const int row = row0 + wr * WR + 32 * j + (lane & 31);
-    if constexpr (EPI == EPI_STATS) {
-      const int tgt = row < n_valid ? a.tgt[row] : -1;
-      float m = -INFINITY;
+    const int rowb = row0 + wr * WR + 32 * j, row = rowb + (lane & 31);
+    const int r = lane & 31;
+    bool live = true;
+    int tgt = -1;
+    float l2 = 0.0f, l2lo = 0.0f, gl = 0.0f;
+    bool here = false;  // some token's target is among the wave's columns
+    if constexpr (EPI == EPI_GRAD) {
+      live = row < n_valid;
+      if (live) {
+        tgt = a.tgt[row] - a.col0 - cw;
+        gl = a.gl[row];
+        const float lse = a.lse[row];
+        l2 = lse * kLog2e;  // and what it lacks, so that p is not off by the rounding of a large lse
+        l2lo = fmaf(lse, kLog2e, -l2);
+      }
+      here = __any(tgt >= 0 && tgt < WC);
+    }
 #pragma unroll
-      for (int i = 0; i < TC; ++i)
+    for (int i = 0; i < TC; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = cw + 32 * i + 8 * (e >> 2) + hi4 + (e & 3);
-          if (col < a.cols) {
-            m = fmaxf(m, acc[i][j][e]);
-            if (col + a.col0 == tgt) a.tlogit[row] = acc[i][j][e];
+      for (int q = 0; q < 4; ++q) {
+        const int col = cw + 32 * i + 8 * q + hi4;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = acc[i][j][4 * q + e];
+          if constexpr (EPI == EPI_GRAD) x = __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -l2) - l2lo);
+          v[e] = x;
+        }
+        if constexpr (EPI == EPI_GRAD) {
+          if (here) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] -= col - cw + e == tgt ? 1.0f : 0.0f;
+          }
+          v *= gl;
+          if (!live) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = col + e < a.cols ? v[e] : 0.0f;
           }
         }
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float mb = (m == -INFINITY ? 0.0f : m);
-      float s = 0.0f;
+        *reinterpret_cast<f32x4*>(mine + r * WC + ((8 * i + 2 * q + hi) ^ (r & (CH - 1))) * 4) = v;
+      }
+    asm volatile("" ::: "memory");  // LDS operations of a wave are done in order
 #pragma unroll
-      for (int i = 0; i < TC; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = cw + 32 * i + 8 * (e >> 2) + hi4 + (e & 3);
-          if (col < a.cols) s += __builtin_amdgcn_exp2f((acc[i][j][e] - mb) * kLog2e);
+    for (int t = 0; t < 32 / kRowsAt; ++t) {
+      const int rr = t * kRowsAt + lane / CH, c = lane % CH;
+      const int orow = rowb + rr, col = cw + 4 * c;
+      f32x4 v = *reinterpret_cast<const f32x4*>(mine + rr * WC + (c ^ (rr & (CH - 1))) * 4);
+      if constexpr (EPI == EPI_GRAD) {
+        for (int n = 0; n < a.nlimb; ++n) {
+          u32x2 w;
+          w[0] = pack_bf16(v[0], v[1]);
+          w[1] = pack_bf16(v[2], v[3]);
+          *reinterpret_cast<u32x2*>(a.g[n] + static_cast<int64_t>(orow) * a.ldg + col) = w;
+          v[0] -= __uint_as_float(w[0] << 16);
+          v[1] -= __uint_as_float(w[0] & 0xFFFF0000u);
+          v[2] -= __uint_as_float(w[1] << 16);
+          v[3] -= __uint_as_float(w[1] & 0xFFFF0000u);
         }
-      s += __shfl_xor(s, 32, 64);
-      if (lane < 32 && row < n_valid)
-        a.part[(static_cast<int64_t>(a.col0 / BC + ct) * NWC + wc) * a.ldpart + row] = make_float2(m, s);
-    } else if constexpr (EPI == EPI_GRAD) {
-      const bool live = row < n_valid;
-      const int tgt = live ? a.tgt[row] : -1;
-      const float lse = live ? a.lse[row] : 0.0f, gl = live ? a.gl[row] : 0.0f;
-#pragma unroll
-      for (int i = 0; i < TC; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int col = cw + 32 * i + 8 * q + hi4;
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float p = __builtin_amdgcn_exp2f((acc[i][j][4 * q + e] - lse) * kLog2e);
-            if (col + e + a.col0 == tgt) p -= 1.0f;
-            v[e] = live && col + e < a.cols ? p * gl : 0.0f;
-          }
-          for (int n = 0; n < a.nlimb; ++n) {
+      } else if constexpr (EPI == EPI_SLAB) {
+        if (orow < n_valid && col < a.ldslab) {
+          f32x4* o = reinterpret_cast<f32x4*>(a.slab + blockIdx.y * a.slab_stride + static_cast<int64_t>(orow) * a.ldslab + col);
+          if (a.add) v += *o;
+          *o = v;
+        }
+      } else if (orow < a.rows && col < a.cols) {
+        const int64_t at = static_cast<int64_t>(orow) * a.ldo + col;
+        if (a.out_bf16) {
+          uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+          if (a.out_vec) {  // cols % 4 == 0: all four exist
             u32x2 w;
+            if (a.add) {
+              w = *reinterpret_cast<const u32x2*>(o);
+              v[0] += __uint_as_float(w[0] << 16);
+              v[1] += __uint_as_float(w[0] & 0xFFFF0000u);
+              v[2] += __uint_as_float(w[1] << 16);
+              v[3] += __uint_as_float(w[1] & 0xFFFF0000u);
+            }
             w[0] = pack_bf16(v[0], v[1]);
             w[1] = pack_bf16(v[2], v[3]);
-            *reinterpret_cast<u32x2*>(a.g[n] + static_cast<int64_t>(row) * a.ldg + col) = w;
-            v[0] -= __uint_as_float(w[0] << 16);
-            v[1] -= __uint_as_float(w[0] & 0xFFFF0000u);
-            v[2] -= __uint_as_float(w[1] << 16);
-            v[3] -= __uint_as_float(w[1] & 0xFFFF0000u);
+            *reinterpret_cast<u32x2*>(o) = w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < a.cols) o[e] = f32_to_bf16(a.add ? bf16_to_f32(o[e]) + v[e] : v[e]);
+          }
+        } else {
+          float* o = static_cast<float*>(a.out) + at;
+          if (a.out_vec) {
+            f32x4 w = v;
+            if (a.add) w += *reinterpret_cast<const f32x4*>(o);
+            *reinterpret_cast<f32x4*>(o) = w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < a.cols) o[e] = a.add ? o[e] + v[e] : v[e];
           }
         }
-    } else if constexpr (EPI == EPI_SLAB) {
-      if (row < n_valid) {
-        float* o = a.slab + blockIdx.y * a.slab_stride + static_cast<int64_t>(row) * a.ldslab;
-#pragma unroll
-        for (int i = 0; i < TC; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int col = cw + 32 * i + 8 * q + hi4;
-            if (col < a.ldslab) {
-              f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-              if (a.add) v += *reinterpret_cast<const f32x4*>(o + col);
-              *reinterpret_cast<f32x4*>(o + col) = v;
-            }
-          }
-      }
-    } else {
-      if (row < a.rows) {
-#pragma unroll
-        for (int i = 0; i < TC; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int col = cw + 32 * i + 8 * q + hi4;
-            float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-            if (a.out_bf16) {
-              uint16_t* o = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(row) * a.ldo + col;
-              if (a.out_vec && col < a.cols) {  // cols % 4 == 0: all four exist
-                u32x2 w;
-                if (a.add) {
-                  w = *reinterpret_cast<const u32x2*>(o);
-                  v[0] += __uint_as_float(w[0] << 16);
-                  v[1] += __uint_as_float(w[0] & 0xFFFF0000u);
-                  v[2] += __uint_as_float(w[1] << 16);
-                  v[3] += __uint_as_float(w[1] & 0xFFFF0000u);
-                }
-                w[0] = pack_bf16(v[0], v[1]);
-                w[1] = pack_bf16(v[2], v[3]);
-                *reinterpret_cast<u32x2*>(o) = w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (col + e < a.cols) o[e] = f32_to_bf16(a.add ? bf16_to_f32(o[e]) + v[e] : v[e]);
-              }
-            } else {
-              float* o = static_cast<float*>(a.out) + static_cast<int64_t>(row) * a.ldo + col;
-              if (a.out_vec && col < a.cols) {
-                f32x4 w = {v[0], v[1], v[2], v[3]};
-                if (a.add) w += *reinterpret_cast<const f32x4*>(o);
-                *reinterpret_cast<f32x4*>(o) = w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (col + e < a.cols) o[e] = a.add ? o[e] + v[e] : v[e];
-              }
-            }
-          }
       }
     }
+    asm volatile("" ::: "memory");
   }
 }

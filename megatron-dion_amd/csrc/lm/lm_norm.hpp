@@ -46,21 +46,41 @@ __device__ __forceinline__ float e4m3_clamp(float v) {  // NaN stays NaN
   return v > 448.0f ? 448.0f : v < -448.0f ? -448.0f : v;
 }
 
+// round_e4m3(v inv), VEC bytes
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t* y, const float* v, float inv) {
+  if constexpr (VEC == 1) {
+    *y = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[0] * inv), 0.0f, 0, false) & 0xFF);
+  } else {
+    u32x2 q;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[4 * k] * inv), e4m3_clamp(v[4 * k + 1] * inv), 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[4 * k + 2] * inv), e4m3_clamp(v[4 * k + 3] * inv), w, true);
+      q[k] = static_cast<uint32_t>(w);
+    }
+    *reinterpret_cast<u32x2*>(y) = q;
+  }
+}
+
+// The 8-bit output's scales: blocks of columns that neighbouring lanes hold, or any blocks (through LDS).
+enum { Q8_NONE = 0, Q8_LANES = 1, Q8_ANY = 2 };
+
 // threads of a block: 4 rows of 64 threads, or one row of LPR
 template <int LPR>
 constexpr int norm_threads() { return LPR > 64 ? LPR : 256; }
 
-template <typename T, int VEC, int LPR, int NV, bool QUANT>
+template <typename T, int VEC, int LPR, int NV, int Q8>
 __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const NormArgs a) {
   constexpr int RPB = LPR > 64 ? 1 : 4;
   __shared__ float red[16];
-  extern __shared__ uint32_t amax[];  // QUANT: sblocks words for each row of the block
+  extern __shared__ uint32_t amax[];  // Q8_ANY: sblocks words for each row of the block
   const int t = LPR > 64 ? threadIdx.x : (threadIdx.x & 63);
   const int sub = LPR > 64 ? 0 : (threadIdx.x >> 6);
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + sub;
   const bool live = row < a.rows;  // whole waves: RPB == 4 has a row for each wave
   float v[NV][VEC];
-  if constexpr (QUANT) {
+  if constexpr (Q8 == Q8_ANY) {
     for (int i = t; i < a.sblocks; i += LPR) amax[sub * a.sblocks + i] = 0u;
     __syncthreads();
   }
@@ -116,11 +136,32 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
         load_weight<VEC>(a, c, w);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) v[i][k] = v[i][k] * rstd * w[k];
-        if constexpr (!QUANT) store_vec<VEC>(static_cast<T*>(a.y) + row * a.ldy + c, v[i]);
+        if constexpr (Q8 == Q8_NONE) store_vec<VEC>(static_cast<T*>(a.y) + row * a.ldy + c, v[i]);
       }
     }
   }
-  if constexpr (QUANT) {
+  if constexpr (Q8 == Q8_LANES) {
+    // a scale's columns are those of 2^n neighbouring lanes of a wave (sblock = 8 .. 512)
+    const int span = a.sblock >> 3, shift = 31 - __clz(a.sblock);
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LPR + t) * VEC;
+        float m = 0.0f;
+        if (c < a.cols) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) m = fmaxf(m, fabsf(v[i][k]));  // passes over NaN
+        }
+        for (int o = 1; o < span; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float s = fmaxf(m / 448.0f, 1.17549435e-38f), inv = 1.0f / s;
+        if (c < a.cols) {
+          if ((t & (span - 1)) == 0) a.scale[row * a.sblocks + (c >> shift)] = s;
+          store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + row * a.ldy + c, v[i], inv);
+        }
+      }
+    }
+  }
+  if constexpr (Q8 == Q8_ANY) {
     // |y| as bits is ordered like an integer; a maximum does not depend on the order it is taken in
     if (live) {
 #pragma unroll
@@ -144,13 +185,11 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
       for (int i = 0; i < NV; ++i) {
         const int c = (i * LPR + t) * VEC;
         if (c < a.cols) {
-          uint8_t b[VEC];
 #pragma unroll
           for (int k = 0; k < VEC; ++k) {
             const float s = fmaxf(__uint_as_float(amax[sub * a.sblocks + (c + k) / a.sblock]) / 448.0f, 1.17549435e-38f);
-            b[k] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[i][k] / s), 0.0f, 0, false) & 0xFF);
+            store_e4m3<1>(y + c + k, &v[i][k], 1.0f / s);
           }
-          for (int k = 0; k < VEC; ++k) y[c + k] = b[k];
         }
       }
     }
@@ -177,13 +216,14 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const Nor
   if (a.dropping) key = philox_key(a.drop);
   for (int64_t row = first; row < a.rows; row += step) {
     const float rstd = a.rstd[row];
-    float u[NV][VEC], g[NV][VEC], dot = 0.0f;  // u = h rstd, g = gy then w gy
+    float u[NV][VEC], g[NV][VEC], q[NV][VEC], dot = 0.0f;  // u = h rstd, g = gy then w gy
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LPR + t) * VEC;
       if (c < a.cols) {
         load_vec<VEC>(static_cast<const T*>(a.h_in) + row * a.ldh + c, u[i]);
         load_vec<VEC>(static_cast<const T*>(a.gy) + row * a.ldgy + c, g[i]);
+        if (a.gh) load_vec<VEC>(static_cast<const T*>(a.gh) + row * a.ldgh + c, q[i]);
       }
     }
 #pragma unroll
@@ -209,10 +249,8 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const Nor
 #pragma unroll
           for (int k = 0; k < VEC; ++k) d[k] = rstd * (g[i][k] - u[i][k] * mean);
           if (a.gh) {
-            float q[VEC];
-            load_vec<VEC>(static_cast<const T*>(a.gh) + row * a.ldgh + c, q);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) d[k] += q[k];
+            for (int k = 0; k < VEC; ++k) d[k] += q[i][k];
           }
           if (a.gr) store_vec<VEC>(static_cast<T*>(a.gr) + row * a.ldgr + c, d);
           if (a.gx) {
@@ -233,17 +271,28 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const Nor
   }
 }
 
-// grad_weight = the sum of the partials in a fixed order: 32 columns a block, 8 threads a column
-__global__ void __launch_bounds__(256) norm_dw_kernel(const NormArgs a, int parts) {
-  __shared__ float red[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+// grad_weight = the sum of the partials in a fixed order: 16 columns a block, 64 threads a column,
+// four partials in flight a thread
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const NormArgs a, int parts) {
+  __shared__ float red[64][17];
+  const int x = threadIdx.x & 15, k = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
   float s = 0.0f;
-  if (c < a.cols)
-    for (int i = k; i < parts; i += 8) s += a.part[static_cast<int64_t>(i) * a.cols + c];
-  red[k][threadIdx.x & 31] = s;
-  __syncthreads();
+  if (c < a.cols) {
+    const float* p = a.part + c;
+    int i = k;
+    for (; i + 192 < parts; i += 256)
+      s += (p[static_cast<int64_t>(i) * a.cols] + p[static_cast<int64_t>(i + 64) * a.cols]) +
+           (p[static_cast<int64_t>(i + 128) * a.cols] + p[static_cast<int64_t>(i + 192) * a.cols]);
+    for (; i < parts; i += 64) s += p[static_cast<int64_t>(i) * a.cols];
+  }
+  red[k][x] = s;
+#pragma unroll
+  for (int half = 32; half > 0; half >>= 1) {
+    __syncthreads();
+    if (k < half) red[k][x] += red[k + half][x];
+  }
   if (k == 0 && c < a.cols) {
-    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x & 31];
+    s = red[0][x];
     if (a.gw_bf16) {
       uint16_t* o = static_cast<uint16_t*>(a.gw) + c;
       *o = f32_to_bf16(a.accumulate ? bf16_to_f32(*o) + s : s);
@@ -258,11 +307,11 @@ namespace rms {
 
 constexpr int kMaxCols = 16384;
 
-// partials of grad_weight: blocks of the backward kernel (two for each CU: every one reads the
-// weight once and leaves one partial row), times the rows that a block works on at once
+// Blocks of the backward kernel, each of which leaves one partial row of grad_weight (four, where a
+// row is a wave's): four for each CU.
 long bwd_blocks(int64_t rows, bool wave_rows) {
   const long want = wave_rows ? ceil_div(rows, 4) : rows;
-  return want < 512 ? (want < 1 ? 1 : want) : 512;
+  return want < 1024 ? (want < 1 ? 1 : want) : 1024;
 }
 bool wave_rows(int cols, bool vec) { return vec ? cols <= 1024 : cols <= 512; }
 
@@ -271,13 +320,13 @@ size_t ws_bytes(const DionNormDesc* d) {  // the larger of the two layouts: alig
   return sizeof(float) * static_cast<size_t>(a > b ? a : b) * d->cols;
 }
 
-template <typename T, bool QUANT>
+template <typename T, int Q8>
 int forward(const NormArgs& a, bool vec, hipStream_t st) {
 #define DION_NORM_FWD(VEC, LPR, NV)                                                                            \
   do {                                                                                                         \
     constexpr int RPB = LPR > 64 ? 1 : 4;                                                                      \
-    const size_t lds = QUANT ? sizeof(uint32_t) * RPB * a.sblocks : 0;                                         \
-    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, LPR, NV, QUANT>), dim3(ceil_div(a.rows, RPB)),                 \
+    const size_t lds = Q8 == Q8_ANY ? sizeof(uint32_t) * RPB * a.sblocks : 0;                                         \
+    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, LPR, NV, Q8>), dim3(ceil_div(a.rows, RPB)),                 \
                        dim3(norm_threads<LPR>()), lds, st, a);                                                 \
   } while (0)
   if (vec) {
@@ -287,7 +336,7 @@ int forward(const NormArgs& a, bool vec, hipStream_t st) {
     else if (a.cols <= 4096) DION_NORM_FWD(8, 256, 2);
     else if (a.cols <= 8192) DION_NORM_FWD(8, 512, 2);
     else DION_NORM_FWD(8, 1024, 2);
-  } else {
+  } else if constexpr (Q8 != Q8_LANES) {
     if (a.cols <= 512) DION_NORM_FWD(1, 64, 8);
     else if (a.cols <= 1024) DION_NORM_FWD(1, 256, 4);
     else if (a.cols <= 4096) DION_NORM_FWD(1, 256, 16);
@@ -319,7 +368,7 @@ int backward(const NormArgs& a, bool vec, hipStream_t st) {
 #undef DION_NORM_BWD
   int rc = check_launch("rms_norm_add_backward");
   if (rc != DION_OK || a.gw == nullptr) return rc;
-  hipLaunchKernelGGL(norm_dw_kernel, dim3(ceil_div(a.cols, 32)), dim3(256), 0, st, a,
+  hipLaunchKernelGGL(norm_dw_kernel, dim3(ceil_div(a.cols, 16)), dim3(1024), 0, st, a,
                      static_cast<int>(blocks * (wr ? 4 : 1)));
   return check_launch("rms_norm_add_backward(weight)");
 }

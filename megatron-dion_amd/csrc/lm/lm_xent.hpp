@@ -1,8 +1,8 @@
 // lm_xent.hpp -- the linear cross entropy: tokens that take part, limbs, the pieces of the vocabulary.
 //
-// forward   select -> pack X -> [pack W] logits tiles, each leaving (max, sum of exp) of its columns
+// forward   select, pack X [, pack W] -> logits tiles, each leaving (maximum, sum of exp) of its columns
 //           for each token -> join them: lse, loss
-// backward  select -> pack X -> for each piece of the vocabulary: [pack W], logits again, g = the
+// backward  select, pack X -> for each piece of the vocabulary: [pack W], logits again, g = the
 //           gradient of the logits to the workspace, dX += g W, dW = g^T X -> round dX
 //
 // Only tokens with a target (and, backward, a gradient) take part: select numbers them, pack X
@@ -26,25 +26,27 @@ struct Tokens {  // compact arrays, by the number a token has among those that t
   float* tlogit; // [tokens_p] (forward)
 };
 
-// One block: numbers the tokens that take part, in order.
-__global__ void __launch_bounds__(1024) select_kernel(const int64_t* target, const float* lse, const float* gl,
-                                                      int tokens, int64_t ignore, int64_t start, int64_t vocab,
-                                                      int64_t total, Tokens o) {
+struct SelectArgs {
+  const int64_t* target;
+  const float *lse, *gl;  // backward
+  int tokens;
+  int64_t ignore, start, vocab, total;
+  Tokens out;
+};
+
+// Numbers the tokens that take part, in order; the whole block (1024 threads) takes part.
+// f(t, n): token t (this thread's) has the number n, -1: none.  Returns how many there are.
+template <typename F>
+__device__ __forceinline__ int select(const SelectArgs& a, F&& f) {
   __shared__ int wsum[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int t0 = 0; t0 < tokens; t0 += 1024) {
+  for (int t0 = 0; t0 < a.tokens; t0 += 1024) {
     const int t = t0 + threadIdx.x;
-    int64_t y = 0;
-    float g = 0.0f;
     bool in = false;
-    if (t < tokens) {
-      y = target[t];
-      in = y != ignore;
-      if (gl) {
-        g = gl[t];
-        in = in && !(g == 0.0f);  // NaN takes part
-      }
+    if (t < a.tokens) {
+      in = a.target[t] != a.ignore;
+      if (a.gl) in = in && !(a.gl[t] == 0.0f);  // NaN takes part
     }
     const uint64_t mask = __ballot(in);
     if (lane == 0) wsum[wave] = __popcll(mask);
@@ -54,23 +56,32 @@ __global__ void __launch_bounds__(1024) select_kernel(const int64_t* target, con
       if (w < wave) before += wsum[w];
       all += wsum[w];
     }
-    if (in) {
-      const int n = before + __popcll(mask & ((1ull << lane) - 1));
-      const bool known = y >= 0 && y < total;
-      o.index[n] = t;
-      o.tgt[n] = known && y >= start && y < start + vocab ? static_cast<int>(y - start) : -1;
-      if (gl) {
-        o.gl[n] = known ? g : NAN;  // a target that is no word: the gradient says so
-        o.lse[n] = lse[t];
-      } else {
-        o.tlogit[n] = known ? 0.0f : NAN;
-      }
-    }
-    if (t < tokens) o.pos[t] = in ? before + __popcll(mask & ((1ull << lane) - 1)) : -1;
+    if (t < a.tokens) f(t, in ? before + __popcll(mask & ((1ull << lane) - 1)) : -1);
     base += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) *o.count = base;
+  return base;
+}
+
+// What the products need to know of token t, whose number is n.
+__device__ __forceinline__ void put_token(const SelectArgs& a, int t, int n) {
+  a.out.pos[t] = n;
+  if (n < 0) return;
+  const int64_t y = a.target[t];
+  const bool known = y >= 0 && y < a.total;  // a target that is no word: loss and gradient say so
+  a.out.index[n] = t;
+  a.out.tgt[n] = known && y >= a.start && y < a.start + a.vocab ? static_cast<int>(y - a.start) : -1;
+  if (a.gl) {
+    a.out.gl[n] = known ? a.gl[t] : NAN;
+    a.out.lse[n] = a.lse[t];
+  } else {
+    a.out.tlogit[n] = known ? 0.0f : NAN;
+  }
+}
+
+__global__ void __launch_bounds__(1024) select_kernel(const SelectArgs a) {
+  const int n = select(a, [&](int t, int k) { put_token(a, t, k); });
+  if (threadIdx.x == 0) *a.out.count = n;
 }
 
 struct PackArgs {
@@ -80,69 +91,104 @@ struct PackArgs {
   const int* count;    // with index: rows that exist
   int rows, cols;      // source extents
   int rows_p, cols_p;  // packed extents, zeros outside the source
-  uint16_t* dst[3];
+  uint16_t* dst;       // limbs one after the other
   int nlimb, vec;
 };
 
-// rows of src as bf16 limbs, 8 columns a thread
+// 8 columns of a row of src as bf16 limbs, `i`: which
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
-  const int rows = a.index ? *a.count : a.rows;
+__device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, const int* index) {
   const int per = a.cols_p / 8;
-  const int64_t n = static_cast<int64_t>(a.rows_p) * per;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int row = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(row) * per) * 8;
-    float v[8];
+  const int row = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(row) * per) * 8;
+  float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    if (row < rows) {
-      const T* s = static_cast<const T*>(a.src) + static_cast<int64_t>(a.index ? a.index[row] : row) * a.ld + c;
-      if (a.vec && c + 8 <= a.cols) {
-        load_vec<8>(s, v);
-      } else {
+  for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+  if (row < rows) {
+    const T* s = static_cast<const T*>(a.src) + static_cast<int64_t>(index ? index[row] : row) * a.ld + c;
+    if (a.vec && c + 8 <= a.cols) {
+      load_vec<8>(s, v);
+    } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (c + k < a.cols) v[k] = to_f32(s[k]);
-      }
+      for (int k = 0; k < 8; ++k)
+        if (c + k < a.cols) v[k] = to_f32(s[k]);
     }
-    for (int l = 0; l < a.nlimb; ++l) {
-      u32x4 q;
+  }
+  uint16_t* o = a.dst + static_cast<int64_t>(row) * a.cols_p + c;
+  for (int l = 0; l < a.nlimb; ++l) {
+    u32x4 q;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        q[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
-        v[2 * k] -= __uint_as_float(q[k] << 16);
-        v[2 * k + 1] -= __uint_as_float(q[k] & 0xFFFF0000u);
-      }
-      *reinterpret_cast<u32x4*>(a.dst[l] + static_cast<int64_t>(row) * a.cols_p + c) = q;
+    for (int k = 0; k < 4; ++k) {
+      q[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
+      v[2 * k] -= __uint_as_float(q[k] << 16);
+      v[2 * k + 1] -= __uint_as_float(q[k] & 0xFFFF0000u);
     }
+    *reinterpret_cast<u32x4*>(o) = q;
+    o += static_cast<int64_t>(a.rows_p) * a.cols_p;
   }
 }
 
-// Joins the tiles' (max, sum): 32 tokens a block, 8 threads a token.
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+  const int rows = a.index ? *a.count : a.rows;
+  const int64_t n = static_cast<int64_t>(a.rows_p) * (a.cols_p / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
+    pack8<T>(a, i, rows, a.index);
+}
+
+// select and both packs in one launch, for few tokens: every block numbers the tokens for itself (a
+// round or two of 1024), the first one writes it down.  x: hidden states, w: the weight's piece (0 rows: none).
+constexpr int kFewTokens = 2048;
+
+template <typename T>
+__global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const PackArgs x, const PackArgs w) {
+  __shared__ int index[kFewTokens];
+  const int count = select(a, [&](int t, int n) {
+    if (n >= 0) index[n] = t;
+    if (blockIdx.x == 0) put_token(a, t, n);
+  });
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.out.count = count;
+  const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), nw = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + nw;
+       i += static_cast<int64_t>(gridDim.x) * 1024) {
+    if (i < nx) pack8<T>(x, i, count, index);
+    else pack8<T>(w, i - nx, w.rows, nullptr);
+  }
+}
+
+// (c, sum of 2^(x log2(e) - c)) of two sets of logits; an empty set (c = -inf) has the sum 0 (or NaN)
+__device__ __forceinline__ float2 join2(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), mb = m == -INFINITY ? 0.0f : m;
+  return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - mb) + b.y * __builtin_amdgcn_exp2f(b.x - mb));
+}
+
+// Joins the tiles' (c, sum): TB tokens a block, 256 / TB threads a token, four parts in flight a thread.
+template <int TB>
 __global__ void __launch_bounds__(256) join_kernel(const float2* part, int parts, int64_t ldpart, int tokens, Tokens o,
                                                    float* loss, float* lse, float* tlogit) {
-  __shared__ float2 red[8][32];
-  const int t = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+  constexpr int NT = 256 / TB;
+  __shared__ float2 red[NT][TB];
+  const int t = blockIdx.x * TB + threadIdx.x % TB, k = threadIdx.x / TB;
   const int n = t < tokens ? o.pos[t] : -1;
-  float m = -INFINITY, s = 0.0f;
+  float2 v = make_float2(-INFINITY, 0.0f);
   if (n >= 0) {
-    for (int i = k; i < parts; i += 8) {
-      const float2 p = part[static_cast<int64_t>(i) * ldpart + n];
-      const float mn = fmaxf(m, p.x), mb = mn == -INFINITY ? 0.0f : mn;
-      s = s * __builtin_amdgcn_exp2f((m - mb) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mb) * kLog2e);
-      m = mn;
+    const float2* p = part + n;
+    int i = k;
+    for (; i + 3 * NT < parts; i += 4 * NT) {
+      const float2 a = p[i * ldpart], b = p[(i + NT) * ldpart], c = p[(i + 2 * NT) * ldpart], d = p[(i + 3 * NT) * ldpart];
+      v = join2(v, join2(join2(a, b), join2(c, d)));
     }
+    for (; i < parts; i += NT) v = join2(v, p[i * ldpart]);
   }
-  red[k][threadIdx.x & 31] = make_float2(m, s);
-  __syncthreads();
+  red[k][threadIdx.x % TB] = v;
+#pragma unroll
+  for (int half = NT / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (k < half) red[k][threadIdx.x % TB] = join2(red[k][threadIdx.x % TB], red[k + half][threadIdx.x % TB]);
+  }
   if (k == 0 && t < tokens) {
-    for (int i = 1; i < 8; ++i) {
-      const float2 p = red[i][threadIdx.x & 31];
-      const float mn = fmaxf(m, p.x), mb = mn == -INFINITY ? 0.0f : mn;
-      s = s * __builtin_amdgcn_exp2f((m - mb) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - mb) * kLog2e);
-      m = mn;
-    }
-    const float l = n < 0 ? 0.0f : m + logf(s), z = n < 0 ? 0.0f : o.tlogit[n];
+    const float m = red[0][threadIdx.x].x, s = red[0][threadIdx.x].y;
+    const float l = n < 0 ? 0.0f : fmaf(m, kLn2, logf(s)), z = n < 0 ? 0.0f : o.tlogit[n];
     lse[t] = l;
     if (tlogit) tlogit[t] = z;
     if (loss) loss[t] = l - z;
@@ -173,8 +219,7 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
 struct Plan {
   int limbs_in;   // of X and W
   int limbs_g;
-  int br;         // tile rows of the logits and dX products: 32, 128 or 256
-  int bc;         // tile columns: 128 or 256
+  int logits, dx, dw;  // tiles of the products (kTiles)
   int tokens_p, hidden_p;
   bool pack_w;
   int piece;      // vocabulary rows of a piece (multiple of 256)
@@ -192,15 +237,40 @@ bool w_direct(const DionXentDesc* d) {
   return d->dtype == DION_DTYPE_BF16 && d->hidden % 8 == 0 && d->ld_weight % 8 == 0 && !d->pack_weight;
 }
 
+// The tiles there are: rows x columns, and the columns of a wave (the logits leave one (max, sum) for
+// each of them).
+struct TileShape {
+  int br, bc, wc;
+};
+constexpr TileShape kTiles[4] = {{64, 64, 32}, {64, 128, 64}, {128, 128, 64}, {256, 256, 128}};
+
+// The largest tile that makes `parts` x `rows` x `cols` into enough blocks for 256 CUs, and that the rows
+// fill.  Measured (us, tile 256 / 128 / 64x128 / 64; blocks of the first):
+//   logits   8192 tokens x 32000 words, h 4096: 907 (2000 blocks) / 1074 / 1470 / 1767 at 4096 tokens;
+//            122 (250) / 148 / 188 / 222 at 512;  106 (125) / 78 / 102 / 114 at 256;
+//            91 / 60 / 55 / 68 at 128;  89 / 58 / 49 / 54 at 1
+//   fp32, 154 of 513 tokens x 5003 words, h 1000: 135 / 78 / 68 / 71
+//   dX       (splits of k make up for few tiles) 1759 / 2010 / 2720 / 3865 at 4096 tokens, 177 / 180 / 204 / 236
+//            at 256, 164 / 132 / 144 / 146 at 128 (with their logits)
+//   dW       324 / 330 / 388 / 417 at 512 tokens, 253 / 234 / 271 / 289 at 256, 65 / 45 / 38 / 35 where it
+//            has 16 / 64 / 128 / 256 blocks (2000 words, h 512; all with their logits)
+int pick_tile(long rows, long cols, long parts, int most) {
+  const long blocks[4] = {0, 128, 256, 192};
+  for (int t = most; t > 0; --t)
+    if (ceil_div(rows, kTiles[t].br) * ceil_div(cols, kTiles[t].bc) * parts >= blocks[t]) return t;
+  return 0;
+}
+
 Plan make_plan(const DionXentDesc* d, int op) {
   Plan p;
   memset(&p, 0, sizeof(p));
   const bool f32 = d->dtype == DION_DTYPE_F32;
   p.limbs_in = f32 ? 3 : 1;
   p.limbs_g = f32 || d->gw_dtype == DION_DTYPE_F32 ? 3 : 1;
-  p.br = d->tokens <= 32 ? 32 : d->tokens <= 128 ? 128 : 256;
-  p.bc = p.br == 256 ? 256 : 128;
-  p.tokens_p = static_cast<int>(round_up(d->tokens, p.br < 64 ? 64 : p.br));
+  p.logits = pick_tile(d->tokens, d->vocab, 1, 3);
+  p.dx = pick_tile(d->tokens, d->hidden, ceil_div(d->vocab, 256), d->tokens >= 256 ? 3 : d->tokens > 64 ? 2 : 1);
+  const int br = kTiles[p.logits].br > kTiles[p.dx].br ? kTiles[p.logits].br : kTiles[p.dx].br;
+  p.tokens_p = static_cast<int>(round_up(d->tokens, br));
   p.hidden_p = static_cast<int>(round_up(d->hidden, kBK));
   p.pack_w = f32 || !w_direct(d);
   const long vocab_p = round_up(d->vocab, 256);
@@ -228,12 +298,13 @@ Plan make_plan(const DionXentDesc* d, int op) {
   p.xp = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
   if (p.pack_w) p.wp = take(static_cast<size_t>(p.limbs_in) * p.piece * p.hidden_p * 2);
   if (op == DION_XENT_FORWARD) {
-    const int per = p.bc / (p.br == 256 ? 128 : p.br == 128 ? 64 : 32);
-    p.parts = static_cast<int>(p.pieces * (p.piece / p.bc)) * per;
+    p.parts = p.pieces * (p.piece / kTiles[p.logits].wc);
     p.part = take(static_cast<size_t>(p.parts) * tp * sizeof(float2));
   } else {
-    const long tiles = static_cast<long>(p.tokens_p / p.br > 0 ? p.tokens_p / p.br : 1) * ceil_div(d->hidden, p.bc);
-    const long want = (p.br == 256 ? 256 : 1024) / (tiles < 1 ? 1 : tiles);  // one or four blocks a CU
+    p.dw = pick_tile(p.piece, d->hidden, 1, d->tokens >= 512 ? 3 : 2);
+    const TileShape t = kTiles[p.dx];
+    const long tiles = ceil_div(d->tokens, t.br) * ceil_div(d->hidden, t.bc);
+    const long want = (t.br == 256 ? 256 : t.br == 128 ? 512 : 1024) / tiles;  // as many blocks as fit at once
     const long most = p.piece / 256;
     p.splits = static_cast<int>(want < 1 ? 1 : want > most ? most : want);
     p.g = take(static_cast<size_t>(p.limbs_g) * tp * p.piece * 2);
@@ -273,11 +344,13 @@ int launch_tile(GemmArgs a, long rows, long cols, hipStream_t st, const char* wh
 }
 
 template <bool RKS, bool CKS, int EPI>
-int launch(int br, const GemmArgs& a, long rows, long cols, hipStream_t st, const char* what) {
-  if (br == 256) return launch_tile<256, 256, 64, 128, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
-  if (br == 128) return launch_tile<128, 128, 64, 64, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
-  if constexpr (!RKS) return launch_tile<32, 128, 32, 32, RKS, CKS, EPI, 3>(a, rows, cols, st, what);
-  return fail(DION_E_INVALID, "%s: no tile", what);
+int launch(int tile, const GemmArgs& a, long rows, long cols, hipStream_t st, const char* what) {
+  switch (tile) {
+    case 3: return launch_tile<256, 256, 64, 128, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
+    case 2: return launch_tile<128, 128, 64, 64, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
+    case 1: return launch_tile<64, 128, 32, 64, RKS, CKS, EPI, 3>(a, rows, cols, st, what);
+    default: return launch_tile<64, 64, 32, 32, RKS, CKS, EPI, 3>(a, rows, cols, st, what);
+  }
 }
 
 Tokens tokens_at(char* ws, const Plan& p) {
@@ -294,8 +367,8 @@ Tokens tokens_at(char* ws, const Plan& p) {
   return t;
 }
 
-int pack(const void* src, int dtype, int64_t ld, const int* index, const int* count, int rows, int cols, int rows_p,
-         int cols_p, uint16_t* dst, int nlimb, hipStream_t st, const char* what) {
+PackArgs pack_args(const void* src, int64_t ld, const int* index, const int* count, int rows, int cols, int rows_p,
+                   int cols_p, uint16_t* dst, int nlimb) {
   PackArgs a;
   memset(&a, 0, sizeof(a));
   a.src = src;
@@ -306,17 +379,64 @@ int pack(const void* src, int dtype, int64_t ld, const int* index, const int* co
   a.cols = cols;
   a.rows_p = rows_p;
   a.cols_p = cols_p;
-  for (int l = 0; l < nlimb; ++l) a.dst[l] = dst + static_cast<size_t>(l) * rows_p * cols_p;
+  a.dst = dst;
   a.nlimb = nlimb;
   a.vec = aligned16(src) && ld % 8 == 0;
-  const long blocks = ceil_div(static_cast<long>(rows_p) * (cols_p / 8), 256);
+  return a;
+}
+
+int pack(const PackArgs& a, int dtype, hipStream_t st, const char* what) {
+  const long blocks = ceil_div(static_cast<long>(a.rows_p) * (a.cols_p / 8), 256);
   const dim3 grid(blocks < 8192 ? blocks : 8192);
   if (dtype == DION_DTYPE_F32) hipLaunchKernelGGL(pack_kernel<float>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(pack_kernel<bf16>, grid, dim3(256), 0, st, a);
   return check_launch(what);
 }
 
-// The W operand of a piece that starts at row v0: where it lies, or its limbs in the workspace.
+// The limbs of the weight's rows v0 .. v0 + n in the workspace.
+PackArgs weight_args(const DionXentDesc* d, const Plan& p, const void* weight, int v0, int n, char* ws) {
+  const char* src = static_cast<const char*>(weight) +
+                    static_cast<int64_t>(v0) * d->ld_weight * (d->dtype == DION_DTYPE_F32 ? 4 : 2);
+  return pack_args(src, d->ld_weight, nullptr, nullptr, n, d->hidden, p.piece, p.hidden_p,
+                   reinterpret_cast<uint16_t*>(ws + p.wp), p.limbs_in);
+}
+
+// Numbers the tokens, gathers their hidden states, and packs the weight's first piece where it has to be.
+int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void* weight, const int64_t* target,
+            const float* lse, const float* gl, const Tokens& tok, char* ws, hipStream_t st) {
+  SelectArgs a;
+  memset(&a, 0, sizeof(a));
+  a.target = target;
+  a.lse = lse;
+  a.gl = gl;
+  a.tokens = static_cast<int>(d->tokens);
+  a.ignore = d->ignore_index;
+  a.start = d->vocab_start;
+  a.vocab = d->vocab;
+  a.total = d->vocab_total;
+  a.out = tok;
+  const PackArgs x = pack_args(hidden, d->ld_hidden, tok.index, tok.count, p.tokens_p, d->hidden, p.tokens_p,
+                               p.hidden_p, reinterpret_cast<uint16_t*>(ws + p.xp), p.limbs_in);
+  PackArgs w;
+  memset(&w, 0, sizeof(w));
+  w.cols_p = 8;
+  if (p.pack_w) w = weight_args(d, p, weight, 0, d->vocab < p.piece ? d->vocab : p.piece, ws);
+  if (d->tokens <= kFewTokens) {
+    const long blocks = ceil_div(static_cast<long>(x.rows_p) * (x.cols_p / 8) + static_cast<long>(w.rows_p) * (w.cols_p / 8), 1024);
+    const dim3 grid(blocks < 1024 ? blocks : 1024);
+    if (d->dtype == DION_DTYPE_F32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(1024), 0, st, a, x, w);
+    else hipLaunchKernelGGL(prepare_kernel<bf16>, grid, dim3(1024), 0, st, a, x, w);
+    return check_launch("xent(prepare)");
+  }
+  hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a);
+  int rc = check_launch("xent(select)");
+  if (rc == DION_OK) rc = pack(x, d->dtype, st, "xent(pack hidden)");
+  if (rc == DION_OK && p.pack_w) rc = pack(w, d->dtype, st, "xent(pack weight)");
+  return rc;
+}
+
+// The W operand of a piece that starts at row v0: where it lies, or its limbs in the workspace (the
+// first piece's are there already).
 int piece_w(const DionXentDesc* d, const Plan& p, const void* weight, int v0, int n, char* ws, const uint16_t** w,
             int64_t* ld, size_t* stride, hipStream_t st) {
   if (!p.pack_w) {
@@ -325,14 +445,10 @@ int piece_w(const DionXentDesc* d, const Plan& p, const void* weight, int v0, in
     *stride = 0;
     return DION_OK;
   }
-  uint16_t* dst = reinterpret_cast<uint16_t*>(ws + p.wp);
-  const int esz = d->dtype == DION_DTYPE_F32 ? 4 : 2;
-  const char* src = static_cast<const char*>(weight) + static_cast<int64_t>(v0) * d->ld_weight * esz;
-  *w = dst;
+  *w = reinterpret_cast<uint16_t*>(ws + p.wp);
   *ld = p.hidden_p;
   *stride = static_cast<size_t>(p.piece) * p.hidden_p;
-  return pack(src, d->dtype, d->ld_weight, nullptr, nullptr, n, d->hidden, p.piece, p.hidden_p, dst, p.limbs_in, st,
-              "xent(pack weight)");
+  return v0 == 0 ? DION_OK : pack(weight_args(d, p, weight, v0, n, ws), d->dtype, st, "xent(pack weight)");
 }
 
 void logits_args(GemmArgs* a, const DionXentDesc* d, const Plan& p, const uint16_t* x, const uint16_t* w, int64_t ldw,
@@ -355,12 +471,7 @@ int forward(const DionXentDesc* d, const void* hidden, const void* weight, const
   const Plan p = make_plan(d, DION_XENT_FORWARD);
   const Tokens tok = tokens_at(ws, p);
   uint16_t* x = reinterpret_cast<uint16_t*>(ws + p.xp);
-  hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, target, nullptr, nullptr, static_cast<int>(d->tokens),
-                     d->ignore_index, d->vocab_start, static_cast<int64_t>(d->vocab), d->vocab_total, tok);
-  int rc = check_launch("xent(select)");
-  if (rc != DION_OK) return rc;
-  rc = pack(hidden, d->dtype, d->ld_hidden, tok.index, tok.count, p.tokens_p, d->hidden, p.tokens_p, p.hidden_p, x,
-            p.limbs_in, st, "xent(pack hidden)");
+  int rc = prepare(d, p, hidden, weight, target, nullptr, nullptr, tok, ws, st);
   if (rc != DION_OK) return rc;
   float2* part = reinterpret_cast<float2*>(ws + p.part);
   for (int v0 = 0; v0 < d->vocab; v0 += p.piece) {
@@ -375,14 +486,19 @@ int forward(const DionXentDesc* d, const void* hidden, const void* weight, const
     a.part = part;
     a.ldpart = p.tokens_p;
     a.tlogit = tok.tlogit;
-    rc = launch<false, false, EPI_STATS>(p.br, a, d->tokens, n, st, "xent(logits)");
+    rc = launch<false, false, EPI_STATS>(p.logits, a, d->tokens, n, st, "xent(logits)");
     if (rc != DION_OK) return rc;
   }
   // tiles that exist, the last piece's ragged one among them
-  const int per = p.bc / (p.br == 256 ? 128 : p.br == 128 ? 64 : 32);
-  const int parts = static_cast<int>(ceil_div(d->vocab, p.bc)) * per;
-  hipLaunchKernelGGL(join_kernel, dim3(ceil_div(d->tokens, 32)), dim3(256), 0, st, part, parts,
-                     static_cast<int64_t>(p.tokens_p), static_cast<int>(d->tokens), tok, loss, lse, tlogit);
+  const int parts = static_cast<int>(ceil_div(d->vocab, kTiles[p.logits].bc)) * (kTiles[p.logits].bc / kTiles[p.logits].wc);
+  // neighbouring tokens share cache lines, but few tokens need all the threads
+#define DION_JOIN(TB)                                                                                      \
+  hipLaunchKernelGGL(join_kernel<TB>, dim3(ceil_div(d->tokens, TB)), dim3(256), 0, st, part, parts,        \
+                     static_cast<int64_t>(p.tokens_p), static_cast<int>(d->tokens), tok, loss, lse, tlogit)
+  if (d->tokens >= 4096) DION_JOIN(16);
+  else if (d->tokens >= 512) DION_JOIN(8);
+  else DION_JOIN(1);
+#undef DION_JOIN
   return check_launch("xent(join)");
 }
 
@@ -394,12 +510,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
   uint16_t* g = reinterpret_cast<uint16_t*>(ws + p.g);
   float* slab = reinterpret_cast<float*>(ws + p.slab);
   const size_t gstride = static_cast<size_t>(p.tokens_p) * p.piece, xstride = static_cast<size_t>(p.tokens_p) * p.hidden_p;
-  hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, target, lse, grad_loss, static_cast<int>(d->tokens),
-                     d->ignore_index, d->vocab_start, static_cast<int64_t>(d->vocab), d->vocab_total, tok);
-  int rc = check_launch("xent(select)");
-  if (rc != DION_OK) return rc;
-  rc = pack(hidden, d->dtype, d->ld_hidden, tok.index, tok.count, p.tokens_p, d->hidden, p.tokens_p, p.hidden_p, x,
-            p.limbs_in, st, "xent(pack hidden)");
+  int rc = prepare(d, p, hidden, weight, target, lse, grad_loss, tok, ws, st);
   if (rc != DION_OK) return rc;
   const int gw_size = d->gw_dtype == DION_DTYPE_F32 ? 4 : 2;
   for (int v0 = 0; v0 < d->vocab; v0 += p.piece) {
@@ -416,7 +527,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     for (int l = 0; l < p.limbs_g; ++l) a.g[l] = g + l * gstride;
     a.nlimb = p.limbs_g;
     a.ldg = p.piece;
-    rc = launch<false, false, EPI_GRAD>(p.br, a, p.tokens_p, n, st, "xent(logit gradients)");
+    rc = launch<false, false, EPI_GRAD>(p.logits, a, p.tokens_p, n, st, "xent(logit gradients)");
     if (rc != DION_OK) return rc;
     if (grad_hidden) {
       memset(&a, 0, sizeof(a));
@@ -432,7 +543,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.ldslab = p.hidden_p;
       a.slab_stride = static_cast<int64_t>(p.tokens_p) * p.hidden_p;
       a.add = v0 > 0;
-      rc = launch<false, true, EPI_SLAB>(p.br, a, d->tokens, d->hidden, st, "xent(grad hidden)");
+      rc = launch<false, true, EPI_SLAB>(p.dx, a, d->tokens, d->hidden, st, "xent(grad hidden)");
       if (rc != DION_OK) return rc;
     }
     if (grad_weight) {
@@ -450,8 +561,9 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.ldo = d->ld_grad_weight;
       a.out_bf16 = gw_size == 2;
       a.out_vec = d->hidden % 4 == 0 && d->ld_grad_weight % 4 == 0 && aligned16(grad_weight);
-      // a piece of g is made of whole tiles, so its rows past n hold zeros; 256-row tiles stay inside it
-      rc = launch<true, true, EPI_OUT>(p.br == 256 ? 256 : 128, a, n, d->hidden, st, "xent(grad weight)");
+      // tiles stay inside the piece of g (a multiple of 256 words): what lies past n there makes rows
+      // that are not stored
+      rc = launch<true, true, EPI_OUT>(p.dw, a, n, d->hidden, st, "xent(grad weight)");
       if (rc != DION_OK) return rc;
     }
   }
