@@ -204,7 +204,7 @@ int dion_xent_workspace_bytes(const DionXentDesc* d, int op, size_t* bytes) {
   const int rc = check_xent(d, op);
   if (rc != DION_OK) return rc;
   if (bytes == nullptr) return fail(DION_E_INVALID, "null bytes");
-  *bytes = xent::make_plan(d, op).total;
+  *bytes = d->tokens == 0 ? 0 : xent::make_plan(d, op).total;
   return DION_OK;
 }
 

@@ -40,7 +40,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss, lse = lm_ops.linear_cross_entropy_forward(hidden, weight, target, **kwargs)
         ctx.save_for_backward(hidden, weight, target, lse)
         ctx.kwargs, ctx.main_grad = kwargs, main_grad
-        return loss.clone() if loss._base is not None else loss
+        return loss
 
     @staticmethod
     @once_differentiable

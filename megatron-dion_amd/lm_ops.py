@@ -16,6 +16,7 @@ leading axes evenly strided (what `view(-1, cols)` accepts); anything else raise
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -29,6 +30,7 @@ __all__ = ["linear_cross_entropy_forward", "linear_cross_entropy_backward", "rms
 Rng = Union[Tuple[int, int], torch.Tensor]
 _U64 = (1 << 64) - 1
 _CODE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_byref = ctypes.byref
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -38,62 +40,53 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _matrix(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """`t` as (rows, cols) without a copy; its device, shape and dtype checked against `like`."""
-    if t.dim() == 0:
+def _rows(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """(rows, cols, row stride) of `t` read as a matrix, without a copy."""
+    shape = t.shape
+    if not shape:
         raise RuntimeError(f"[DION_BAD_SHAPE] {what} has no axis")
     if not t.is_cuda:
         raise RuntimeError(f"[DION_BAD_DEVICE] {what} is on {t.device}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+    cols = shape[-1]
+    if t.is_contiguous():
+        return (t.numel() // cols if cols else 0), cols, cols
+    strides = t.stride()
+    rows, ld, ok = 1, 0, cols <= 1 or strides[-1] == 1
+    for n, st in zip(reversed(shape[:-1]), reversed(strides[:-1])):  # the leading axes have to fold into one
+        if n != 1:
+            ok = ok and (st == rows * ld if ld else st >= cols)
+            ld = ld or st
+            rows *= n
+    if not ok and t.numel():
+        raise RuntimeError(f"[DION_NON_ROW_MAJOR] {what}: shape={tuple(shape)} stride={strides}")
+    return rows, cols, ld or cols
+
+
+def _like(t: torch.Tensor, what: str, like: torch.Tensor) -> int:
+    """The row stride of `t`, which has to be a tensor like `like`."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] {what}: {tuple(t.shape)} {t.dtype} {t.device}, expected "
                            f"{tuple(like.shape)} {like.dtype} {like.device}")
-    cols = t.shape[-1]
-    if t.dim() == 2 and (t.stride(1) == 1 or cols <= 1) and (t.stride(0) >= cols or t.shape[0] <= 1):
-        return t
-    if t.is_contiguous():
-        return t.view(t.numel() // cols if cols else 0, cols)
-    try:
-        v = t.view(-1, cols) if t.numel() else t.reshape(-1, max(cols, 1))
-    except RuntimeError:
-        v = None
-    if v is None or (cols > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < cols):
-        raise RuntimeError(f"[DION_NON_ROW_MAJOR] {what}: shape={tuple(t.shape)} stride={t.stride()}")
-    return v
+    return _rows(t, what)[2]
 
 
-def _ld(m: torch.Tensor) -> int:
-    return int(m.stride(0)) if m.shape[0] > 1 else max(int(m.shape[1]), 1)
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _stream(device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-class _on:
-    """The device that a call's kernels are launched on (no change when it is the current one)."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.guard = None
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(fn, device: torch.device, *args) -> int:
+    """`fn(*args, stream)` on the current stream of `device`, which need not be the current device."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor:
     # a call's own memory, from the caching allocator: calls on different streams and captured graphs
     # never share it
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes if nbytes > 16 else 16, dtype=torch.uint8, device=device)
 
 
 def _rng(p: float, rng: Optional[Rng], device) -> Optional[_lm_lib.DionRng]:
@@ -113,7 +106,7 @@ def _rng(p: float, rng: Optional[Rng], device) -> Optional[_lm_lib.DionRng]:
 
 
 def _ref(s):
-    return None if s is None else ctypes.byref(s)
+    return None if s is None else _byref(s)
 
 
 # ------------------------------------------------------------------------------- dropout
@@ -126,17 +119,16 @@ def dropout_add_forward(x: torch.Tensor, residual: Optional[torch.Tensor] = None
     infinity).  `rng` is `(seed, offset)`, or an int64 tensor holding them on x's device, which a
     captured graph reads again at each replay.  A (seed, offset) pair is to be used for one mask only:
     count `offset` over layers, steps and ranks."""
-    xm = _matrix(x, "x")
-    rm = None if residual is None else _matrix(residual, "residual", x)
+    rows, cols, ld = _rows(x, "x")
+    ld_r = 0 if residual is None else _like(residual, "residual", x)
     code = _dtype(x, "x")
-    r = _rng(p, rng, x.device)
-    lib = _lm_lib.load()
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _on(x.device):
-        rc = lib.dion_dropout_add(xm.shape[0], xm.shape[1], code, xm.data_ptr(), _ld(xm), _ptr(rm),
-                                  0 if rm is None else _ld(rm), out.data_ptr(), max(int(xm.shape[1]), 1), float(p),
-                                  _ref(r), _stream(x.device))
-    _lm_lib.check(rc, "dion_dropout_add")
+    device = x.device
+    r = _rng(p, rng, device)
+    out = _empty(x)
+    rc = _call(_lm_lib.load().dion_dropout_add, device, rows, cols, code, x.data_ptr(), ld,
+               None if residual is None else residual.data_ptr(), ld_r, out.data_ptr(), cols, p, _ref(r))
+    if rc:
+        _lm_lib.check(rc, "dion_dropout_add")
     return out
 
 
@@ -160,18 +152,21 @@ class RmsNormAddGrads(NamedTuple):
     grad_weight: Optional[torch.Tensor]
 
 
-def _norm_desc(xm: torch.Tensor, weight: torch.Tensor, p: float) -> _lm_lib.DionNormDesc:
-    if weight.dim() != 1 or weight.shape[0] != xm.shape[1] or weight.device != xm.device or \
-            not weight.is_contiguous():
+@functools.lru_cache(maxsize=512)
+def _norm_desc(rows, cols, dtype, w_dtype, gw_dtype, y_dtype, scale_block, accumulate, eps, p, *lds):
+    """The descriptor of a call (read only: calls of the same shapes share it) and its scratch."""
+    d = _lm_lib.DionNormDesc(rows, cols, dtype, w_dtype, gw_dtype, y_dtype, scale_block, accumulate, eps, p, *lds)
+    nbytes = ctypes.c_size_t(0)
+    _lm_lib.check(_lm_lib.load().dion_rms_norm_add_workspace_bytes(_byref(d), _byref(nbytes)),
+                  "dion_rms_norm_add_workspace_bytes")
+    return d, int(nbytes.value)
+
+
+def _norm_weight(weight: torch.Tensor, cols: int, device) -> int:
+    if weight.shape != (cols,) or weight.device != device or not weight.is_contiguous():
         raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] weight: {tuple(weight.shape)} {weight.device}, expected "
-                           f"({xm.shape[1]},) on {xm.device}")
-    d = _lm_lib.DionNormDesc()
-    d.rows, d.cols = int(xm.shape[0]), int(xm.shape[1])
-    d.dtype, d.w_dtype = _dtype(xm, "x"), _dtype(weight, "weight")
-    d.gw_dtype = d.w_dtype
-    d.y_dtype = d.dtype
-    d.p = float(p)
-    return d
+                           f"({cols},) on {device}")
+    return _dtype(weight, "weight")
 
 
 def rms_norm_add_forward(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
@@ -182,32 +177,29 @@ def rms_norm_add_forward(x: torch.Tensor, weight: torch.Tensor, residual: Option
     `scale_block` > 0 (at least 8, or all columns; -1: one block a row): y is float8_e4m3fn, each block
     of that many columns over its own fp32 `scale` = max |y| / 448 (at least 2^-126), so that
     `y.float() * scale` restores it.  Dropout as in `dropout_add_forward`."""
-    xm = _matrix(x, "x")
-    rm = None if residual is None else _matrix(residual, "residual", x)
-    d = _norm_desc(xm, weight, p)
-    d.eps = float(eps)
-    r = _rng(p, rng, x.device)
-    rows, cols = int(d.rows), int(d.cols)
-    lib = _lm_lib.load()
-    stored = rm is not None or p > 0.0
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if stored else x
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    scale = None
+    rows, cols, ld = _rows(x, "x")
+    ld_r = 0 if residual is None else _like(residual, "residual", x)
+    device = x.device
+    code, w_code = _dtype(x, "x"), _norm_weight(weight, cols, device)
+    r = _rng(p, rng, device)
+    stored = residual is not None or r is not None
+    shape = x.shape[:-1]
     if scale_block:
-        d.y_dtype = _lm_lib.DTYPE_E4M3
-        d.scale_block = cols if scale_block < 0 or scale_block > cols else int(scale_block)
-        scale = torch.empty(tuple(x.shape[:-1]) + (-(-cols // max(d.scale_block, 1)),), dtype=torch.float32,
-                            device=x.device)
-        y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        block = cols if scale_block < 0 or scale_block > cols else int(scale_block)
+        d, _ = _norm_desc(rows, cols, code, w_code, w_code, _lm_lib.DTYPE_E4M3, block, 0, float(eps), float(p),
+                          ld, ld_r, cols, cols)
+        scale = torch.empty(shape + (-(-cols // block),), dtype=torch.float32, device=device)
+        y = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
     else:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    d.ld_x, d.ld_residual = _ld(xm), 0 if rm is None else _ld(rm)
-    d.ld_h = d.ld_y = cols
-    with _on(x.device):
-        rc = lib.dion_rms_norm_add(ctypes.byref(d), xm.data_ptr(), _ptr(rm), weight.data_ptr(),
-                                   h.data_ptr() if stored else None, y.data_ptr(), _ptr(scale), rstd.data_ptr(),
-                                   _ref(r), _stream(x.device))
-    _lm_lib.check(rc, "dion_rms_norm_add")
+        d, _ = _norm_desc(rows, cols, code, w_code, w_code, code, 0, 0, float(eps), float(p), ld, ld_r, cols, cols)
+        scale, y = None, _empty(x)
+    h = _empty(x) if stored else x
+    rstd = torch.empty(shape, dtype=torch.float32, device=device)
+    rc = _call(_lm_lib.load().dion_rms_norm_add, device, _byref(d), x.data_ptr(),
+               None if residual is None else residual.data_ptr(), weight.data_ptr(), h.data_ptr() if stored else None,
+               y.data_ptr(), None if scale is None else scale.data_ptr(), rstd.data_ptr(), _ref(r))
+    if rc:
+        _lm_lib.check(rc, "dion_rms_norm_add")
     return RmsNormAdd(y, h, rstd, scale)
 
 
@@ -215,7 +207,7 @@ def _grad_weight(weight: torch.Tensor, out: Optional[torch.Tensor], accumulate: 
     if out is None:
         if accumulate:
             raise RuntimeError(f"[DION_BAD_GRAD_OUT] accumulate needs {what}")
-        return torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+        return _empty(weight)
     if out.shape != weight.shape or out.device != weight.device:
         raise RuntimeError(f"[DION_BAD_GRAD_OUT] {what}: {tuple(out.shape)} {out.device}, expected "
                            f"{tuple(weight.shape)} {weight.device}")
@@ -230,72 +222,73 @@ def rms_norm_add_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.T
     stream's gradient), `p` and `rng` are the forward's.  An 8-bit y passes `grad_y` (x's dtype) as if
     it had not been rounded.  `grad_weight` (fp32 or bf16, e.g. `weight.main_grad`) is written, or with
     `accumulate` added to; without it a new tensor of weight's dtype is returned."""
-    hm = _matrix(h, "h")
-    gm = _matrix(grad_y, "grad_y", h)
-    ghm = None if grad_h is None else _matrix(grad_h, "grad_h", h)
-    d = _norm_desc(hm, weight, p)
-    r = _rng(p, rng, h.device)
-    if rstd.dtype != torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous() or \
-            rstd.device != h.device:
-        raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] rstd: {tuple(rstd.shape)} {rstd.dtype}")
-    cols = int(d.cols)
+    rows, cols, ld = _rows(h, "h")
+    ld_gy = _like(grad_y, "grad_y", h)
+    ld_gh = 0 if grad_h is None else _like(grad_h, "grad_h", h)
+    device = h.device
+    code, w_code = _dtype(h, "h"), _norm_weight(weight, cols, device)
+    r = _rng(p, rng, device)
+    if rstd.dtype != torch.float32 or rstd.shape != h.shape[:-1] or not rstd.is_contiguous() or rstd.device != device:
+        raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] rstd: {tuple(rstd.shape)} {rstd.dtype} {rstd.device}")
     gx = gr = gw = ws = None
-    if need_input:
-        gx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-        if p > 0.0:
-            gr = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    lib = _lm_lib.load()
+    gw_code = w_code
     if need_weight:
         gw = _grad_weight(weight, grad_weight, accumulate, "grad_weight")
         if not gw.is_contiguous():
             raise RuntimeError(f"[DION_BAD_GRAD_OUT] grad_weight stride={gw.stride()}")
-        d.gw_dtype = _dtype(gw, "grad_weight")
-        d.accumulate = int(bool(accumulate))
-        nbytes = ctypes.c_size_t(0)
-        _lm_lib.check(lib.dion_rms_norm_add_workspace_bytes(ctypes.byref(d), ctypes.byref(nbytes)),
-                      "dion_rms_norm_add_workspace_bytes")
-        ws = _workspace(nbytes.value, h.device)
-    d.ld_h, d.ld_grad_y, d.ld_grad_h = _ld(hm), _ld(gm), 0 if ghm is None else _ld(ghm)
-    d.ld_grad_x = d.ld_grad_residual = cols
-    with _on(h.device):
-        rc = lib.dion_rms_norm_add_backward(ctypes.byref(d), gm.data_ptr(), hm.data_ptr(), weight.data_ptr(),
-                                            rstd.data_ptr(), _ptr(ghm), _ptr(gx), _ptr(gr), _ptr(gw), _ref(r),
-                                            _ptr(ws), 0 if ws is None else ws.numel(), _stream(h.device))
-    _lm_lib.check(rc, "dion_rms_norm_add_backward")
+        gw_code = _dtype(gw, "grad_weight")
+    d, nbytes = _norm_desc(rows, cols, code, w_code, gw_code, code, 0, int(bool(accumulate)), 0.0, float(p), 0, 0, ld, 0,
+                           ld_gy, ld_gh, cols, cols)
+    if need_input:
+        gx = _empty(h)
+        if r is not None:
+            gr = _empty(h)
+    if need_weight:
+        ws = _workspace(nbytes, device)
+    rc = _call(_lm_lib.load().dion_rms_norm_add_backward, device, _byref(d), grad_y.data_ptr(), h.data_ptr(),
+               weight.data_ptr(), rstd.data_ptr(), None if grad_h is None else grad_h.data_ptr(),
+               None if gx is None else gx.data_ptr(), None if gr is None else gr.data_ptr(),
+               None if gw is None else gw.data_ptr(), _ref(r), None if ws is None else ws.data_ptr(),
+               0 if ws is None else nbytes if nbytes > 16 else 16)
+    if rc:
+        _lm_lib.check(rc, "dion_rms_norm_add_backward")
     return RmsNormAddGrads(gx, gx if gr is None else gr, gw)
 
 
 # ------------------------------------------------------------------------------- linear cross entropy
-def _xent_desc(hidden, weight, target, vocab_start, vocab_size, ignore_index, op):
-    hm = _matrix(hidden, "hidden")
-    wm = _matrix(weight, "weight")
-    if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or weight.dtype != hidden.dtype or \
-            weight.device != hidden.device:
+@functools.lru_cache(maxsize=512)
+def _xent_shape(op, tokens, hidden, vocab, dtype, gw_dtype, accumulate, pack_weight, start, total, ignore, ld_hidden,
+                ld_weight, ld_grad_weight, piece_bytes):
+    """The descriptor of a call (read only: calls of the same shapes share it) and its scratch."""
+    d = _lm_lib.DionXentDesc(tokens, hidden, vocab, dtype, gw_dtype, accumulate, pack_weight, start, total, ignore,
+                             ld_hidden, ld_weight, hidden, ld_grad_weight, piece_bytes)
+    nbytes = ctypes.c_size_t(0)
+    _lm_lib.check(_lm_lib.load().dion_xent_workspace_bytes(_byref(d), op, _byref(nbytes)),
+                  "dion_xent_workspace_bytes")
+    return d, int(nbytes.value)
+
+
+def _xent_desc(op, hidden, weight, target, vocab_start, vocab_size, ignore_index, grad_weight=None, accumulate=False,
+               piece_bytes=0):
+    tokens, cols, ld_h = _rows(hidden, "hidden")
+    if weight.dim() != 2 or weight.shape[1] != cols or weight.dtype != hidden.dtype or weight.device != hidden.device:
         raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] hidden {tuple(hidden.shape)} {hidden.dtype} {hidden.device}, "
                            f"weight {tuple(weight.shape)} {weight.dtype} {weight.device}")
+    rows, _, ld_w = _rows(weight, "weight")
     if target.dtype != torch.int64 or target.shape != hidden.shape[:-1] or target.device != hidden.device:
         raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] target: int64 {tuple(hidden.shape[:-1])} on {hidden.device} "
                            f"expected, got {target.dtype} {tuple(target.shape)} {target.device}")
-    d = _lm_lib.DionXentDesc()
-    d.dtype = _dtype(hidden, "hidden")
-    start, rows = int(vocab_start), int(weight.shape[0])
+    code = _dtype(hidden, "hidden")
+    start = int(vocab_start)
     total = start + rows if vocab_size is None else int(vocab_size)
     if start < 0 or rows < 1 or total <= start:
         raise RuntimeError(f"[DION_BAD_VOCAB] weight of {rows} rows from word {start} on, of {total}")
-    d.tokens, d.hidden = int(hm.shape[0]), int(hm.shape[1])
-    d.vocab = min(rows, total - start)  # rows past the vocabulary are padding
-    d.vocab_start, d.vocab_total, d.ignore_index = start, total, int(ignore_index)
-    d.ld_hidden, d.ld_weight = _ld(hm), _ld(wm)
-    d.gw_dtype = d.dtype
-    d.pack_weight = int(wm.data_ptr() % 16 != 0)
-    return d, hm, wm, target.contiguous().view(-1)
-
-
-def _xent_workspace(lib, d, op, device):
-    nbytes = ctypes.c_size_t(0)
-    _lm_lib.check(lib.dion_xent_workspace_bytes(ctypes.byref(d), op, ctypes.byref(nbytes)),
-                  "dion_xent_workspace_bytes")
-    return _workspace(nbytes.value, device)
+    vocab = min(rows, total - start)  # rows past the vocabulary are padding
+    gw_code, ld_gw = code, cols
+    if grad_weight is not None:
+        gw_code, ld_gw = _dtype(grad_weight, "grad_weight"), _rows(grad_weight, "grad_weight")[2]
+    return _xent_shape(op, tokens, cols, vocab, code, gw_code, int(bool(accumulate)), int(weight.data_ptr() % 16 != 0),
+                       start, total, int(ignore_index), ld_h, ld_w, ld_gw, int(piece_bytes))
 
 
 def combine_vocab_shards(lse: torch.Tensor, tlogit: torch.Tensor, ignored: torch.Tensor, group):
@@ -323,22 +316,21 @@ def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, tar
     Vocabulary shards (tensor parallel): weight holds the rows from `vocab_start` on of a vocabulary of
     `vocab_size` words (rows past it are padding), `group` the ranks that share it; every rank passes the
     same hidden states and targets and gets the whole vocabulary's loss."""
-    d, hm, wm, tv = _xent_desc(hidden, weight, target, vocab_start, vocab_size, ignore_index, _lm_lib.XENT_FORWARD)
-    dev = hidden.device
-    lib = _lm_lib.load()
-    ws = _xent_workspace(lib, d, _lm_lib.XENT_FORWARD, dev)
-    out = torch.empty((2,) + tuple(target.shape), dtype=torch.float32, device=dev)
-    loss, lse = out[0], out[1]
-    with _on(dev):
-        if group is None:
-            rc = lib.dion_xent_forward(ctypes.byref(d), hm.data_ptr(), wm.data_ptr(), tv.data_ptr(), loss.data_ptr(),
-                                       lse.data_ptr(), None, ws.data_ptr(), ws.numel(), _stream(dev))
-            _lm_lib.check(rc, "dion_xent_forward")
-            return loss, lse
-        tlogit = loss
-        rc = lib.dion_xent_forward(ctypes.byref(d), hm.data_ptr(), wm.data_ptr(), tv.data_ptr(), None,
-                                   lse.data_ptr(), tlogit.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
+    d, nbytes = _xent_desc(_lm_lib.XENT_FORWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index)
+    device = hidden.device
+    target = target.contiguous()
+    ws = _workspace(nbytes, device)
+    loss = torch.empty(target.shape, dtype=torch.float32, device=device)
+    lse = torch.empty_like(loss)
+    tlogit = loss if group is not None else None
+    rc = _call(_lm_lib.load().dion_xent_forward, device, _byref(d), hidden.data_ptr(), weight.data_ptr(),
+               target.data_ptr(), loss.data_ptr() if tlogit is None else None, lse.data_ptr(),
+               None if tlogit is None else tlogit.data_ptr(), ws.data_ptr(), ws.numel())
+    if rc:
         _lm_lib.check(rc, "dion_xent_forward")
+    if group is None:
+        return loss, lse
+    with torch.cuda.device(device):
         return combine_vocab_shards(lse, tlogit, target == ignore_index, group)
 
 
@@ -355,32 +347,27 @@ def linear_cross_entropy_backward(grad_loss: torch.Tensor, hidden: torch.Tensor,
     e.g. `weight.main_grad`) is written, or with `accumulate` added to, rows past `vocab_size` as zeros;
     without it a new tensor of weight's dtype is returned.  The logits' gradient is rounded to bf16 for
     the matrix cores where the result is bf16, and split into three bf16 limbs (24 bits) where it is fp32.  With `group`, grad_hidden is summed over the vocabulary's shards."""
-    d, hm, wm, tv = _xent_desc(hidden, weight, target, vocab_start, vocab_size, ignore_index, _lm_lib.XENT_BACKWARD)
+    gw = _grad_weight(weight, grad_weight, accumulate, "grad_weight") if need_weight else None
+    d, nbytes = _xent_desc(_lm_lib.XENT_BACKWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index, gw,
+                           accumulate, piece_bytes)
+    device = hidden.device
     for t, what in ((grad_loss, "grad_loss"), (lse, "lse")):
-        if t.dtype != torch.float32 or t.shape != target.shape or t.device != hidden.device:
+        if t.dtype != torch.float32 or t.shape != target.shape or t.device != device:
             raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] {what}: fp32 {tuple(target.shape)} expected, got "
                                f"{t.dtype} {tuple(t.shape)} {t.device}")
-    dev = hidden.device
-    gl, ls = grad_loss.contiguous(), lse.contiguous()
-    gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if need_hidden else None
-    gw = None
-    if need_weight:
-        gw = _grad_weight(weight, grad_weight, accumulate, "grad_weight")
-        d.gw_dtype = _dtype(gw, "grad_weight")
-        d.ld_grad_weight = _ld(_matrix(gw, "grad_weight"))
-        d.accumulate = int(bool(accumulate))
-        if not accumulate and (d.tokens == 0 or d.vocab < weight.shape[0]):
-            (gw if d.tokens == 0 else gw[d.vocab:]).zero_()
+    gh = _empty(hidden) if need_hidden else None
+    if gw is not None and not accumulate and (d.tokens == 0 or d.vocab < weight.shape[0]):
+        (gw if d.tokens == 0 else gw[d.vocab:]).zero_()
     if d.tokens == 0 or (gh is None and gw is None):
         return gh, gw
-    d.ld_grad_hidden = int(d.hidden)
-    d.piece_bytes = int(piece_bytes)
-    lib = _lm_lib.load()
-    ws = _xent_workspace(lib, d, _lm_lib.XENT_BACKWARD, dev)
-    with _on(dev):
-        rc = lib.dion_xent_backward(ctypes.byref(d), hm.data_ptr(), wm.data_ptr(), tv.data_ptr(), ls.data_ptr(),
-                                    gl.data_ptr(), _ptr(gh), _ptr(gw), ws.data_ptr(), ws.numel(), _stream(dev))
+    target, grad_loss, lse = target.contiguous(), grad_loss.contiguous(), lse.contiguous()
+    ws = _workspace(nbytes, device)
+    rc = _call(_lm_lib.load().dion_xent_backward, device, _byref(d), hidden.data_ptr(), weight.data_ptr(),
+               target.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), None if gh is None else gh.data_ptr(),
+               None if gw is None else gw.data_ptr(), ws.data_ptr(), ws.numel())
+    if rc:
         _lm_lib.check(rc, "dion_xent_backward")
-        if group is not None and gh is not None:
+    if group is not None and gh is not None:
+        with torch.cuda.device(device):
             dist.all_reduce(gh, op=dist.ReduceOp.SUM, group=group)
     return gh, gw

@@ -323,8 +323,9 @@ def test_xent_vocabulary_shards_and_padding(dtype, out_dtype):
     lib = lm_ops
     parts = []
     for k in (0, 256):
-        d, hm, wm, tv = lib._xent_desc(x.cuda(), pad[k:k + 256].cuda(), t.cuda(), k, 500, -100, 1)
-        ws = lib._xent_workspace(lib._lm_lib.load(), d, 1, x.cuda().device)
+        hm, wm, tv = x.cuda(), pad[k:k + 256].cuda(), t.cuda()
+        d, nbytes = lib._xent_desc(1, hm, wm, tv, k, 500, -100)
+        ws = lib._workspace(nbytes, hm.device)
         lse, tl = torch.empty(70, device="cuda"), torch.empty(70, device="cuda")
         import ctypes
         rc = lib._lm_lib.load().dion_xent_forward(ctypes.byref(d), hm.data_ptr(), wm.data_ptr(), tv.data_ptr(), None,

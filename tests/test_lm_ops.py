@@ -98,6 +98,10 @@ def test_xent_workspace_is_far_from_the_logits():
     assert n.value < 200 << 20
     assert lib.dion_xent_workspace_bytes(ctypes.byref(d), _lm_lib.XENT_BACKWARD, ctypes.byref(n)) == 0
     assert n.value < 1400 << 20
+    d.tokens = 0
+    for op in (_lm_lib.XENT_FORWARD, _lm_lib.XENT_BACKWARD):
+        assert lib.dion_xent_workspace_bytes(ctypes.byref(d), op, ctypes.byref(n)) == 0 and n.value == 0
+    d.tokens = 8192
     d.piece_bytes = 64 << 20
     assert lib.dion_xent_workspace_bytes(ctypes.byref(d), _lm_lib.XENT_BACKWARD, ctypes.byref(n)) == 0
     assert n.value < 300 << 20
