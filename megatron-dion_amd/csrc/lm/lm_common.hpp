@@ -56,6 +56,24 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return static_cast<uint32_t>(f32_to_bf16(lo)) | (static_cast<uint32_t>(f32_to_bf16(hi)) << 16);
 }
 
+// fp16 halves of a word, rounded to nearest even (subnormals kept)
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const _Float16 h[2] = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+  uint32_t r;
+  __builtin_memcpy(&r, h, 4);
+  return r;
+}
+__device__ __forceinline__ float f16_lo(uint32_t w) {
+  _Float16 h[2];
+  __builtin_memcpy(h, &w, 4);
+  return static_cast<float>(h[0]);
+}
+__device__ __forceinline__ float f16_hi(uint32_t w) {
+  _Float16 h[2];
+  __builtin_memcpy(h, &w, 4);
+  return static_cast<float>(h[1]);
+}
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(bf16 x) { return bf16_to_f32(x.bits); }
 template <typename T>

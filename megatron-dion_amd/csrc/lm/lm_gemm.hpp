@@ -2,7 +2,7 @@
 //
 //   out[row][col] = sum_k R[row][k] C[col][k]
 //
-// Both operands are bf16 in memory.  An operand is K-contiguous (KC: its rows run along k) or
+// Both operands are 16-bit floats in memory.  An operand is K-contiguous (KC: its rows run along k) or
 // K-strided (KS: its rows run along row / col, one row for each k); a KS tile is transposed on its
 // way out of LDS by ds_read_b64_tr_b16, so that no operand is ever transposed in HBM:
 //   logits  z  = X W^T    R = X [t][h]  KC    C = W [v][h]  KC
@@ -11,9 +11,11 @@
 // The C operand is the MFMA's A matrix: a lane then holds 4 consecutive output columns, and the
 // softmax over columns reduces inside a lane.
 //
-// fp32 operands are sums of bf16 limbs (x = x1 + x2 + x3, each the bf16 nearest to what is left, 8
-// bits each); a product of them is a list of segments, the limb pairs that matter, which the loop
-// walks through as if k were that much longer.  Accumulation is fp32 in the MFMA.
+// An operand of fp32 precision is two fp16 limbs of its values times a power of two that brings the
+// largest under 2^15 (x 2^s = hi + lo, 11 bits each, to 2^-22 of x, or 2^-40 of the largest where that
+// is more); a product of two of them is a list of segments, hi lo + lo hi + hi hi (lo lo is below
+// 2^-22), which the loop walks through as if k were three times as long, and a power of two undoes the
+// scales.  bf16 operands are one segment of bf16.  Accumulation is fp32 in the MFMA.
 //
 // Tiles go to LDS by buffer_load_dwordx4 ... lds, NBUF - 1 to NBUF steps of 64 k ahead; rows and columns
 // past the end get an offset past the descriptor's range, which loads zeros.  16-byte chunks are
@@ -21,10 +23,11 @@
 // KS 64-byte slot s of row k at s ^ (k%4 + 4 (k/8 % 2)).
 
 constexpr int kBK = 64;
-constexpr int kMaxSeg = 6;
+constexpr int kMaxSeg = 3;
 constexpr uint32_t kOob = 0x80000000u;  // == num_records: loads zeros
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -43,12 +46,13 @@ struct GemmArgs {
   const int* tgt;        // per compact token: column of its target within the shard, -1: none
   const float* lse;      // per compact token
   const float* gl;       // per compact token: upstream gradient
+  const float* scale;    // device: what undoes the operands' scales, NULL: 1
   int col0;              // first shard column of this piece
   float2* part;          // stats: [part][token] (c, sum of 2^(x log2(e) - c))
   float* tlogit;         // stats: per compact token
   int64_t ldpart;
-  uint16_t* g[3];        // limbs of g
-  int nlimb;
+  uint16_t* gb;          // g in bf16, or NULL
+  uint16_t* gh[2];       // g 2^(13 - e) in two fp16 limbs, 2^e the power of two below |gl|; or NULL
   int64_t ldg;
   float* slab;           // dX: [split][token][ldslab]
   int64_t ldslab, slab_stride;
@@ -201,7 +205,25 @@ __device__ __forceinline__ void each(F&& f) {
 // stands before the last phase: there every wave has its last fragments of this step's tile, so the
 // tile's buffer is free for the step NBUF on, whose loads are issued in between the phase's MFMAs, and
 // the next step's tile has arrived (vmcnt), whose first fragments the phase reads.
-template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, int EPI, int NBUF>
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// 2^e <= |x| < 2^(e + 1) as 2^e (1 for 0, infinities and NaN)
+__device__ __forceinline__ float pow2_below(float x) {
+  const float v = fabsf(x);
+  if (!(v > 0.0f && v <= 3.402823466e38f)) return 1.0f;
+  int e;
+  frexpf(v, &e);
+  return ldexpf(1.0f, e - 1);
+}
+constexpr float kGradScale = 8192.0f;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
+
+template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF>
 __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const GemmArgs a) {
   constexpr int NWR = BR / WR, NWC = BC / WC, NW = NWR * NWC;
   constexpr int TR = WR / 32, TC = WC / 32;
@@ -301,7 +323,7 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
         constexpr int M = decltype(m)::value, i = M / TR, j = M % TR;
         constexpr int NM = TC * TR, NR = TC + TR;
         constexpr int per = (NR + NM - 1) / NM;  // reads after each MFMA until there are none left
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cv[set][i], rv[set][j], acc[i][j], 0, 0, 0);
+        acc[i][j] = mfma<F16>(cv[set][i], rv[set][j], acc[i][j]);
         each<per>([&](auto r) {
           constexpr int Q = M * per + decltype(r)::value;
           if constexpr (Q < NR) read(set ^ 1, std::integral_constant<int, Q>{}, P == 3 ? then : now, (P + 1) & 3);
@@ -321,6 +343,8 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
   const int hi = lane >> 5, hi4 = hi * 4;
   const int cw = c0 + wc * WC;
   const bool whole = c0 + BC <= a.cols;  // no column of the tile is past the end
+  const float scale = a.scale ? *a.scale : 1.0f;
+  const float l2e = kLog2e * scale;      // exact: scale is a power of two
   if constexpr (EPI == EPI_STATS) {
     // Exponentials to base 2: x log2(e) - c is one fma, and c (the rounded maximum) one exact number in
     // both the terms and the result, so that its rounding does not matter.
@@ -340,7 +364,7 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
         for (int i = 0; i < TC; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (32 * i + 8 * (e >> 2) + hi4 + (e & 3) == tgt) a.tlogit[row] = acc[i][j][e];
+            if (32 * i + 8 * (e >> 2) + hi4 + (e & 3) == tgt) a.tlogit[row] = acc[i][j][e] * scale;
       }
       float m = acc[0][j][0];
 #pragma unroll
@@ -348,12 +372,12 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
 #pragma unroll
         for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
       m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float c = m == -INFINITY ? 0.0f : m * kLog2e;
+      const float c = m == -INFINITY ? 0.0f : m * l2e;
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < TC; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e & 3] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], kLog2e, -c));
+        for (int e = 0; e < 16; ++e) s[e & 3] += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], l2e, -c));
       float sum = (s[0] + s[1]) + (s[2] + s[3]);
       sum += __shfl_xor(sum, 32, 64);
       if (lane < 32 && row < n_valid)
@@ -372,13 +396,14 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
     const int r = lane & 31;
     bool live = true;
     int tgt = -1;
-    float l2 = 0.0f, l2lo = 0.0f, gl = 0.0f;
+    float l2 = 0.0f, l2lo = 0.0f, gl = 0.0f, gm = 0.0f;
     bool here = false;  // some token's target is among the wave's columns
     if constexpr (EPI == EPI_GRAD) {
       live = row < n_valid;
       if (live) {
         tgt = a.tgt[row] - a.col0 - cw;
         gl = a.gl[row];
+        gm = gl * (kGradScale / pow2_below(gl));
         const float lse = a.lse[row];
         l2 = lse * kLog2e;  // and what it lacks, so that p is not off by the rounding of a large lse
         l2lo = fmaf(lse, kLog2e, -l2);
@@ -394,7 +419,7 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = acc[i][j][4 * q + e];
-          if constexpr (EPI == EPI_GRAD) x = __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -l2) - l2lo);
+          if constexpr (EPI == EPI_GRAD) x = __builtin_amdgcn_exp2f(fmaf(x, l2e, -l2) - l2lo);
           v[e] = x;
         }
         if constexpr (EPI == EPI_GRAD) {
@@ -402,7 +427,6 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] -= col - cw + e == tgt ? 1.0f : 0.0f;
           }
-          v *= gl;
           if (!live) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           if (!whole) {
 #pragma unroll
@@ -418,15 +442,23 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
       const int orow = rowb + rr, col = cw + 4 * c;
       f32x4 v = *reinterpret_cast<const f32x4*>(mine + rr * WC + (c ^ (rr & (CH - 1))) * 4);
       if constexpr (EPI == EPI_GRAD) {
-        for (int n = 0; n < a.nlimb; ++n) {
+        const int64_t to = static_cast<int64_t>(orow) * a.ldg + col;
+        const float glr = __shfl(gl, rr, 64);  // lane rr has row rr's
+        if (a.gb) {
           u32x2 w;
-          w[0] = pack_bf16(v[0], v[1]);
-          w[1] = pack_bf16(v[2], v[3]);
-          *reinterpret_cast<u32x2*>(a.g[n] + static_cast<int64_t>(orow) * a.ldg + col) = w;
-          v[0] -= __uint_as_float(w[0] << 16);
-          v[1] -= __uint_as_float(w[0] & 0xFFFF0000u);
-          v[2] -= __uint_as_float(w[1] << 16);
-          v[3] -= __uint_as_float(w[1] & 0xFFFF0000u);
+          w[0] = pack_bf16(v[0] * glr, v[1] * glr);
+          w[1] = pack_bf16(v[2] * glr, v[3] * glr);
+          *reinterpret_cast<u32x2*>(a.gb + to) = w;
+        }
+        if (a.gh[0]) {
+          v *= __shfl(gm, rr, 64);
+          u32x2 w;
+          w[0] = pack_f16(v[0], v[1]);
+          w[1] = pack_f16(v[2], v[3]);
+          *reinterpret_cast<u32x2*>(a.gh[0] + to) = w;
+          w[0] = pack_f16(v[0] - f16_lo(w[0]), v[1] - f16_hi(w[0]));
+          w[1] = pack_f16(v[2] - f16_lo(w[1]), v[3] - f16_hi(w[1]));
+          *reinterpret_cast<u32x2*>(a.gh[1] + to) = w;
         }
       } else if constexpr (EPI == EPI_SLAB) {
         if (orow < n_valid && col < a.ldslab) {
@@ -435,6 +467,7 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
           *o = v;
         }
       } else if (orow < a.rows && col < a.cols) {
+        v *= scale;
         const int64_t at = static_cast<int64_t>(orow) * a.ldo + col;
         if (a.out_bf16) {
           uint16_t* o = static_cast<uint16_t*>(a.out) + at;

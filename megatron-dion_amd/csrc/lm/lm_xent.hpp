@@ -9,10 +9,13 @@
 // gathers their rows, and every product runs over that many.  What a hidden state without a target
 // holds is never read.
 //
-// g is rounded to bf16 limbs for the matrix cores: one limb (2^-8) where all outputs are bf16, whose
-// own rounding is as large; three (2^-24) for dW where grad_weight is fp32 (two, 2^-16, measured 2.6e-6 of
-// its 2-norm, twice what an fp32 product is off) and for fp32 inputs, which are split into three limbs
-// themselves (24 bits, the products kept down to 2^-24).
+// Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
+// whose own rounding is as large, and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
+// an fp32 main_grad (three bf16 limbs measured 1.15 times the time of the whole pass, two left 2.6e-6 of
+// the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
+// limbs themselves.  The power of two that brings such an operand into fp16's range comes from its
+// largest finite value; g's is known, |p - [v = y]| <= 1 times the mantissa of the token's gl, whose
+// power of two goes into X (for dW) or is put back at the end (for dX).
 
 namespace xent {
 
@@ -24,7 +27,12 @@ struct Tokens {  // compact arrays, by the number a token has among those that t
   float* lse;    // [tokens_p] (backward)
   float* gl;     // [tokens_p] (backward)
   float* tlogit; // [tokens_p] (forward)
+  float* amax;   // [3][kAmaxBlocks]: largest |X|, |W|, |X| 2^e of a block's share
+  float* scale;  // [4]: kScaleZ ...
 };
+constexpr int kAmaxBlocks = 512;
+// what undoes the scales of z = X W^T, dX = g W (without the token's 2^e), dW = g^T X
+enum { kScaleZ = 0, kScaleDx = 1, kScaleDw = 2 };
 
 struct SelectArgs {
   const int64_t* target;
@@ -79,11 +87,6 @@ __device__ __forceinline__ void put_token(const SelectArgs& a, int t, int n) {
   }
 }
 
-__global__ void __launch_bounds__(1024) select_kernel(const SelectArgs a) {
-  const int n = select(a, [&](int t, int k) { put_token(a, t, k); });
-  if (threadIdx.x == 0) *a.out.count = n;
-}
-
 struct PackArgs {
   const void* src;
   int64_t ld;
@@ -93,11 +96,98 @@ struct PackArgs {
   int rows_p, cols_p;  // packed extents, zeros outside the source
   uint16_t* dst;       // limbs one after the other
   int nlimb, vec;
+  int f16;             // fp16 limbs of the values times `mul` (a parameter), else one bf16
+  int amax;            // f16: which row of Tokens::amax
+  const float* gl;     // not NULL: times the power of two below |gl| of the row's token, too
 };
 
-// 8 columns of a row of src as bf16 limbs, `i`: which
+// 2^s that brings m under 2^15
+__device__ __forceinline__ float scale_of(float m) {
+  if (!(m > 0.0f)) return 1.0f;
+  int e;
+  frexpf(m, &e);  // m < 2^e
+  e = 15 - e;
+  return ldexpf(1.0f, e < -100 ? -100 : e > 100 ? 100 : e);
+}
+
+// the largest of a row of Tokens::amax; the whole block takes part
+__device__ __forceinline__ float block_amax(const float* p, int n) {
+  __shared__ float red[16];
+  float m = 0.0f;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) m = fmaxf(m, p[i]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = red[0];
+  for (int i = 1; i < static_cast<int>(blockDim.x >> 6); ++i) m = fmaxf(m, red[i]);
+  return m;
+}
+
+struct AmaxArgs {
+  const void *x, *w;
+  int64_t ldx, ldw;
+  int tokens, vocab, hidden, vecx, vecw;
+  int want_x, want_w, want_xg;
+  const int64_t* target;
+  const float* gl;
+  int64_t ignore;
+  float* out;  // Tokens::amax
+};
+
 template <typename T>
-__device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, const int* index) {
+__device__ __forceinline__ float amax8(const T* p, int c, int cols, int vec) {
+  float v[8], m = 0.0f;
+  if (vec && c + 8 <= cols) {
+    load_vec<8>(p + c, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(p[c + k]) : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float y = fabsf(v[k]);
+    m = fmaxf(m, y <= 3.402823466e38f ? y : 0.0f);  // the largest finite one
+  }
+  return m;
+}
+
+// Each block's share of the largest |X| (tokens that take part), |X| 2^e and |W|.
+template <typename T>
+__global__ void __launch_bounds__(256) amax_kernel(const AmaxArgs a) {
+  __shared__ float red[4];
+  const int per = (a.hidden + 7) / 8;
+  float mx = 0.0f, mg = 0.0f, mw = 0.0f;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * 256;
+  if (a.want_x || a.want_xg)
+    for (int64_t i = first; i < static_cast<int64_t>(a.tokens) * per; i += step) {
+      const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
+      if (a.target[t] == a.ignore || (a.gl && a.gl[t] == 0.0f)) continue;
+      const float m = amax8(static_cast<const T*>(a.x) + t * a.ldx, c, a.hidden, a.vecx);
+      mx = fmaxf(mx, m);
+      if (a.want_xg) mg = fmaxf(mg, m * pow2_below(a.gl[t]));
+    }
+  if (a.want_w)
+    for (int64_t i = first; i < static_cast<int64_t>(a.vocab) * per; i += step) {
+      const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
+      mw = fmaxf(mw, amax8(static_cast<const T*>(a.w) + t * a.ldw, c, a.hidden, a.vecw));
+    }
+  float v[3] = {mx, mw, mg <= 3.402823466e38f ? mg : 3.402823466e38f};
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v[k] = fmaxf(v[k], __shfl_xor(v[k], o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v[k];
+    __syncthreads();
+    if (threadIdx.x == 0) a.out[k * kAmaxBlocks + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+}
+
+// 8 columns of a row of src, `i`: which; f16: times mul
+template <typename T>
+__device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, const int* index, float mul) {
   const int per = a.cols_p / 8;
   const int row = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(row) * per) * 8;
   float v[8];
@@ -114,45 +204,85 @@ __device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, co
     }
   }
   uint16_t* o = a.dst + static_cast<int64_t>(row) * a.cols_p + c;
-  for (int l = 0; l < a.nlimb; ++l) {
-    u32x4 q;
+  u32x4 q;
+  if (a.f16) {
+    const float e2 = a.gl && row < rows ? pow2_below(a.gl[index[row]]) : 1.0f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      q[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
-      v[2 * k] -= __uint_as_float(q[k] << 16);
-      v[2 * k + 1] -= __uint_as_float(q[k] & 0xFFFF0000u);
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * e2 * mul;  // in this order as the maximum was taken: no overflow
+    for (int l = 0; l < a.nlimb; ++l) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        q[k] = pack_f16(v[2 * k], v[2 * k + 1]);
+        v[2 * k] -= f16_lo(q[k]);
+        v[2 * k + 1] -= f16_hi(q[k]);
+      }
+      *reinterpret_cast<u32x4*>(o) = q;
+      o += static_cast<int64_t>(a.rows_p) * a.cols_p;
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
     *reinterpret_cast<u32x4*>(o) = q;
-    o += static_cast<int64_t>(a.rows_p) * a.cols_p;
+  }
+}
+
+// What undoes the scales (one thread).
+__device__ __forceinline__ void put_scales(float* scale, float mx, float mw, float mg) {
+  scale[kScaleZ] = (1.0f / scale_of(mx)) * (1.0f / scale_of(mw));
+  scale[kScaleDx] = (1.0f / kGradScale) * (1.0f / scale_of(mw));
+  scale[kScaleDw] = (1.0f / kGradScale) * (1.0f / scale_of(mg));
+}
+
+__global__ void __launch_bounds__(1024) select_kernel(const SelectArgs a, int amax_blocks) {
+  const int n = select(a, [&](int t, int k) { put_token(a, t, k); });
+  if (threadIdx.x == 0) *a.out.count = n;
+  if (amax_blocks) {
+    const float mx = block_amax(a.out.amax, amax_blocks), mw = block_amax(a.out.amax + kAmaxBlocks, amax_blocks),
+                mg = block_amax(a.out.amax + 2 * kAmaxBlocks, amax_blocks);
+    if (threadIdx.x == 0) put_scales(a.out.scale, mx, mw, mg);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a, const float* amax, int amax_blocks) {
   const int rows = a.index ? *a.count : a.rows;
+  const float mul = a.f16 ? scale_of(block_amax(amax + a.amax * kAmaxBlocks, amax_blocks)) : 1.0f;
   const int64_t n = static_cast<int64_t>(a.rows_p) * (a.cols_p / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-    pack8<T>(a, i, rows, a.index);
+    pack8<T>(a, i, rows, a.index, mul);
 }
 
-// select and both packs in one launch, for few tokens: every block numbers the tokens for itself (a
-// round or two of 1024), the first one writes it down.  x: hidden states, w: the weight's piece (0 rows: none).
+// select and the packs in one launch, for few tokens: every block numbers the tokens for itself (a round
+// or two of 1024), the first one writes it down.  x: hidden states for z, xg: for dW (fp16), w: the
+// weight's first piece (0 rows: none).
 constexpr int kFewTokens = 2048;
 
 template <typename T>
-__global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const PackArgs x, const PackArgs w) {
+__global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const PackArgs x, const PackArgs xg,
+                                                       const PackArgs w, int amax_blocks) {
   __shared__ int index[kFewTokens];
   const int count = select(a, [&](int t, int n) {
     if (n >= 0) index[n] = t;
     if (blockIdx.x == 0) put_token(a, t, n);
   });
+  float mul[3] = {1.0f, 1.0f, 1.0f};
+  if (amax_blocks) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (k == 2 ? xg.rows_p > 0 : x.f16 != 0) mul[k] = block_amax(a.out.amax + k * kAmaxBlocks, amax_blocks);
+    if (blockIdx.x == 0 && threadIdx.x == 0) put_scales(a.out.scale, mul[0], mul[1], mul[2]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) mul[k] = scale_of(mul[k]);
+  }
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.out.count = count;
-  const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), nw = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + nw;
+  const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), ng = static_cast<int64_t>(xg.rows_p) * (xg.cols_p / 8),
+                nw = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + ng + nw;
        i += static_cast<int64_t>(gridDim.x) * 1024) {
-    if (i < nx) pack8<T>(x, i, count, index);
-    else pack8<T>(w, i - nx, w.rows, nullptr);
+    if (i < nx) pack8<T>(x, i, count, index, mul[0]);
+    else if (i < nx + ng) pack8<T>(xg, i - nx, count, index, mul[2]);
+    else pack8<T>(w, i - nx - ng, w.rows, nullptr, mul[1]);
   }
 }
 
@@ -198,7 +328,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int parts
 // grad_hidden = the sum of the splits' slabs, rounded; zeros where a token takes no part
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(const float* slab, int splits, int64_t stride, int64_t ldslab,
-                                                    const int* pos, int tokens, int cols, T* out, int64_t ldo) {
+                                                    const int* pos, int tokens, int cols, const float* scale,
+                                                    const float* gl, T* out, int64_t ldo) {
   const int per = static_cast<int>((cols + 3) / 4);
   const int64_t n = static_cast<int64_t>(tokens) * per;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -208,6 +339,7 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
     if (p >= 0)
       for (int s = 0; s < splits; ++s)
         v += *reinterpret_cast<const f32x4*>(slab + s * stride + static_cast<int64_t>(p) * ldslab + c);
+    if (p >= 0 && scale) v = v * *scale * pow2_below(gl[p]);  // one after the other: their product may underflow
     T* o = out + static_cast<int64_t>(t) * ldo + c;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -217,17 +349,20 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
 
 // ------------------------------------------------------------------------------- plan
 struct Plan {
-  int limbs_in;   // of X and W
-  int limbs_g;
-  int logits, dx, dw;  // tiles of the products (kTiles)
+  int f32;             // fp32 inputs
+  int wide;            // backward: grad_weight in fp32 precision
+  int limbs_in;        // of X and W
+  int g_arrays;        // backward: 16-bit arrays of g: bf16 (bf16 inputs), fp16 hi and lo (wide)
+  int logits, dx;      // tiles of the products (kTiles); dW's goes by the piece
   int tokens_p, hidden_p;
   bool pack_w;
   int piece;      // vocabulary rows of a piece (multiple of 256)
   int pieces;
   int splits;     // dX: parts of a piece's k
-  int parts;      // forward: (max, sum) pairs of a token
+  int parts;      // forward: (c, sum) pairs of a token
+  int amax_blocks;
   // workspace offsets
-  size_t tok, xp, wp, part, g, slab, total;
+  size_t tok, xp, xg, wp, part, g, slab, total;
 };
 
 constexpr size_t kPieceBytes = size_t(1) << 30;  // g of one piece, unless the caller says less
@@ -264,28 +399,31 @@ int pick_tile(long rows, long cols, long parts, int most) {
 Plan make_plan(const DionXentDesc* d, int op) {
   Plan p;
   memset(&p, 0, sizeof(p));
-  const bool f32 = d->dtype == DION_DTYPE_F32;
-  p.limbs_in = f32 ? 3 : 1;
-  p.limbs_g = f32 || d->gw_dtype == DION_DTYPE_F32 ? 3 : 1;
+  p.f32 = d->dtype == DION_DTYPE_F32;
+  p.wide = op == DION_XENT_BACKWARD && (p.f32 || d->gw_dtype == DION_DTYPE_F32);
+  p.limbs_in = p.f32 ? 2 : 1;
+  p.g_arrays = p.f32 ? 2 : p.wide ? 3 : 1;
   p.logits = pick_tile(d->tokens, d->vocab, 1, 3);
   p.dx = pick_tile(d->tokens, d->hidden, ceil_div(d->vocab, 256), d->tokens >= 256 ? 3 : d->tokens > 64 ? 2 : 1);
   const int br = kTiles[p.logits].br > kTiles[p.dx].br ? kTiles[p.logits].br : kTiles[p.dx].br;
   p.tokens_p = static_cast<int>(round_up(d->tokens, br));
   p.hidden_p = static_cast<int>(round_up(d->hidden, kBK));
-  p.pack_w = f32 || !w_direct(d);
+  p.pack_w = p.f32 || !w_direct(d);
   const long vocab_p = round_up(d->vocab, 256);
   long piece = vocab_p;
   if (op == DION_XENT_BACKWARD) {
     const size_t most = d->piece_bytes > 0 ? static_cast<size_t>(d->piece_bytes) : kPieceBytes;
-    piece = static_cast<long>(most / (static_cast<size_t>(p.limbs_g) * p.tokens_p * 2)) / 256 * 256;
+    piece = static_cast<long>(most / (static_cast<size_t>(p.g_arrays) * p.tokens_p * 2)) / 256 * 256;
     if (p.pack_w && piece > 32768) piece = 32768;
   } else if (p.pack_w) {
     piece = 32768;
   }
   if (piece < 256) piece = 256;
   if (piece > vocab_p) piece = vocab_p;
-  p.pieces = static_cast<int>(ceil_div(d->vocab, piece));
-  p.piece = static_cast<int>(round_up(ceil_div(d->vocab, p.pieces), 256));  // pieces of like size
+  // whole rounds of dW's 256 x 256 tiles over 256 CUs, where a piece has one
+  const long in_round = 256 / ceil_div(d->hidden, 256) * 256;
+  if (op == DION_XENT_BACKWARD && in_round > 0 && piece > in_round && piece < vocab_p) piece = piece / in_round * in_round;
+  p.piece = static_cast<int>(piece);
   p.pieces = static_cast<int>(ceil_div(d->vocab, p.piece));
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -294,20 +432,24 @@ Plan make_plan(const DionXentDesc* d, int op) {
     return o;
   };
   const size_t tp = static_cast<size_t>(p.tokens_p);
-  p.tok = take(256 + 6 * tp * 4);
+  p.tok = take(512 + 3 * kAmaxBlocks * sizeof(float) + 6 * tp * 4);
   p.xp = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
+  if (p.wide) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
+  if (p.f32 || p.wide) {
+    const long units = (d->tokens + (p.f32 ? d->vocab : 0)) * ceil_div(d->hidden, 8);
+    p.amax_blocks = static_cast<int>(units > kAmaxBlocks * 1024L ? kAmaxBlocks : ceil_div(units, 1024));
+  }
   if (p.pack_w) p.wp = take(static_cast<size_t>(p.limbs_in) * p.piece * p.hidden_p * 2);
   if (op == DION_XENT_FORWARD) {
     p.parts = p.pieces * (p.piece / kTiles[p.logits].wc);
     p.part = take(static_cast<size_t>(p.parts) * tp * sizeof(float2));
   } else {
-    p.dw = pick_tile(p.piece, d->hidden, 1, d->tokens >= 512 ? 3 : 2);
     const TileShape t = kTiles[p.dx];
     const long tiles = ceil_div(d->tokens, t.br) * ceil_div(d->hidden, t.bc);
     const long want = (t.br == 256 ? 256 : t.br == 128 ? 512 : 1024) / tiles;  // as many blocks as fit at once
     const long most = p.piece / 256;
     p.splits = static_cast<int>(want < 1 ? 1 : want > most ? most : want);
-    p.g = take(static_cast<size_t>(p.limbs_g) * tp * p.piece * 2);
+    p.g = take(static_cast<size_t>(p.g_arrays) * tp * p.piece * 2);
     p.slab = take(static_cast<size_t>(p.splits) * tp * p.hidden_p * 4);
   }
   p.total = at;
@@ -327,13 +469,13 @@ void segments(GemmArgs* a, const uint16_t* r, size_t rstride, int rlimbs, const 
       }
 }
 
-template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, int EPI, int NBUF>
+template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF>
 int launch_tile(GemmArgs a, long rows, long cols, hipStream_t st, const char* what) {
   a.row_tiles = static_cast<int>(ceil_div(rows, BR));
   a.col_tiles = static_cast<int>(ceil_div(cols, BC));
   constexpr int threads = 64 * (BR / WR) * (BC / WC);
   constexpr size_t lds = static_cast<size_t>(NBUF) * (BR + BC) * kBK * 2;
-  auto* kernel = gemm_kernel<BR, BC, WR, WC, RKS, CKS, EPI, NBUF>;
+  auto* kernel = gemm_kernel<BR, BC, WR, WC, RKS, CKS, F16, EPI, NBUF>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
@@ -343,14 +485,19 @@ int launch_tile(GemmArgs a, long rows, long cols, hipStream_t st, const char* wh
   return check_launch(what);
 }
 
-template <bool RKS, bool CKS, int EPI>
-int launch(int tile, const GemmArgs& a, long rows, long cols, hipStream_t st, const char* what) {
+template <bool RKS, bool CKS, bool F16, int EPI>
+int launch_as(int tile, const GemmArgs& a, long rows, long cols, hipStream_t st, const char* what) {
   switch (tile) {
-    case 3: return launch_tile<256, 256, 64, 128, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
-    case 2: return launch_tile<128, 128, 64, 64, RKS, CKS, EPI, 2>(a, rows, cols, st, what);
-    case 1: return launch_tile<64, 128, 32, 64, RKS, CKS, EPI, 3>(a, rows, cols, st, what);
-    default: return launch_tile<64, 64, 32, 32, RKS, CKS, EPI, 3>(a, rows, cols, st, what);
+    case 3: return launch_tile<256, 256, 64, 128, RKS, CKS, F16, EPI, 2>(a, rows, cols, st, what);
+    case 2: return launch_tile<128, 128, 64, 64, RKS, CKS, F16, EPI, 2>(a, rows, cols, st, what);
+    case 1: return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);
+    default: return launch_tile<64, 64, 32, 32, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);
   }
+}
+template <bool RKS, bool CKS, int EPI>
+int launch(bool f16, int tile, const GemmArgs& a, long rows, long cols, hipStream_t st, const char* what) {
+  return f16 ? launch_as<RKS, CKS, true, EPI>(tile, a, rows, cols, st, what)
+             : launch_as<RKS, CKS, false, EPI>(tile, a, rows, cols, st, what);
 }
 
 Tokens tokens_at(char* ws, const Plan& p) {
@@ -358,7 +505,9 @@ Tokens tokens_at(char* ws, const Plan& p) {
   char* b = ws + p.tok;
   const size_t n = static_cast<size_t>(p.tokens_p);
   t.count = reinterpret_cast<int*>(b);
-  t.pos = reinterpret_cast<int*>(b + 256);
+  t.scale = reinterpret_cast<float*>(b + 256);
+  t.amax = reinterpret_cast<float*>(b + 512);
+  t.pos = reinterpret_cast<int*>(t.amax + 3 * kAmaxBlocks);
   t.index = t.pos + n;
   t.tgt = t.index + n;
   t.lse = reinterpret_cast<float*>(t.tgt + n);
@@ -368,7 +517,7 @@ Tokens tokens_at(char* ws, const Plan& p) {
 }
 
 PackArgs pack_args(const void* src, int64_t ld, const int* index, const int* count, int rows, int cols, int rows_p,
-                   int cols_p, uint16_t* dst, int nlimb) {
+                   int cols_p, uint16_t* dst, int nlimb, bool f16, int amax, const float* gl) {
   PackArgs a;
   memset(&a, 0, sizeof(a));
   a.src = src;
@@ -382,14 +531,17 @@ PackArgs pack_args(const void* src, int64_t ld, const int* index, const int* cou
   a.dst = dst;
   a.nlimb = nlimb;
   a.vec = aligned16(src) && ld % 8 == 0;
+  a.f16 = f16;
+  a.amax = amax;
+  a.gl = gl;
   return a;
 }
 
-int pack(const PackArgs& a, int dtype, hipStream_t st, const char* what) {
+int pack(const PackArgs& a, const Tokens& tok, const Plan& p, hipStream_t st, const char* what) {
   const long blocks = ceil_div(static_cast<long>(a.rows_p) * (a.cols_p / 8), 256);
   const dim3 grid(blocks < 8192 ? blocks : 8192);
-  if (dtype == DION_DTYPE_F32) hipLaunchKernelGGL(pack_kernel<float>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(pack_kernel<bf16>, grid, dim3(256), 0, st, a);
+  if (p.f32) hipLaunchKernelGGL(pack_kernel<float>, grid, dim3(256), 0, st, a, tok.amax, p.amax_blocks);
+  else hipLaunchKernelGGL(pack_kernel<bf16>, grid, dim3(256), 0, st, a, tok.amax, p.amax_blocks);
   return check_launch(what);
 }
 
@@ -398,7 +550,7 @@ PackArgs weight_args(const DionXentDesc* d, const Plan& p, const void* weight, i
   const char* src = static_cast<const char*>(weight) +
                     static_cast<int64_t>(v0) * d->ld_weight * (d->dtype == DION_DTYPE_F32 ? 4 : 2);
   return pack_args(src, d->ld_weight, nullptr, nullptr, n, d->hidden, p.piece, p.hidden_p,
-                   reinterpret_cast<uint16_t*>(ws + p.wp), p.limbs_in);
+                   reinterpret_cast<uint16_t*>(ws + p.wp), p.limbs_in, p.f32, 1, nullptr);
 }
 
 // Numbers the tokens, gathers their hidden states, and packs the weight's first piece where it has to be.
@@ -415,30 +567,63 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   a.vocab = d->vocab;
   a.total = d->vocab_total;
   a.out = tok;
+  if (p.amax_blocks) {
+    AmaxArgs m;
+    memset(&m, 0, sizeof(m));
+    m.x = hidden;
+    m.w = weight;
+    m.ldx = d->ld_hidden;
+    m.ldw = d->ld_weight;
+    m.tokens = a.tokens;
+    m.vocab = d->vocab;
+    m.hidden = d->hidden;
+    m.vecx = aligned16(hidden) && d->ld_hidden % 8 == 0;
+    m.vecw = aligned16(weight) && d->ld_weight % 8 == 0;
+    m.want_x = m.want_w = p.f32;
+    m.want_xg = p.wide;
+    m.target = target;
+    m.gl = gl;
+    m.ignore = d->ignore_index;
+    m.out = tok.amax;
+    if (p.f32) hipLaunchKernelGGL(amax_kernel<float>, dim3(p.amax_blocks), dim3(256), 0, st, m);
+    else hipLaunchKernelGGL(amax_kernel<bf16>, dim3(p.amax_blocks), dim3(256), 0, st, m);
+    const int rc = check_launch("xent(amax)");
+    if (rc != DION_OK) return rc;
+  }
   const PackArgs x = pack_args(hidden, d->ld_hidden, tok.index, tok.count, p.tokens_p, d->hidden, p.tokens_p,
-                               p.hidden_p, reinterpret_cast<uint16_t*>(ws + p.xp), p.limbs_in);
-  PackArgs w;
+                               p.hidden_p, reinterpret_cast<uint16_t*>(ws + p.xp), p.limbs_in, p.f32, 0, nullptr);
+  PackArgs xg, w;
+  memset(&xg, 0, sizeof(xg));
   memset(&w, 0, sizeof(w));
-  w.cols_p = 8;
+  xg.cols_p = w.cols_p = 8;
+  if (p.wide) {
+    xg = x;
+    xg.dst = reinterpret_cast<uint16_t*>(ws + p.xg);
+    xg.f16 = 1;
+    xg.amax = 2;
+    xg.gl = gl;
+  }
   if (p.pack_w) w = weight_args(d, p, weight, 0, d->vocab < p.piece ? d->vocab : p.piece, ws);
   if (d->tokens <= kFewTokens) {
-    const long blocks = ceil_div(static_cast<long>(x.rows_p) * (x.cols_p / 8) + static_cast<long>(w.rows_p) * (w.cols_p / 8), 1024);
-    const dim3 grid(blocks < 1024 ? blocks : 1024);
-    if (d->dtype == DION_DTYPE_F32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(1024), 0, st, a, x, w);
-    else hipLaunchKernelGGL(prepare_kernel<bf16>, grid, dim3(1024), 0, st, a, x, w);
+    const long units = static_cast<long>(x.rows_p + xg.rows_p) * (x.cols_p / 8) + static_cast<long>(w.rows_p) * (w.cols_p / 8);
+    const long blocks = ceil_div(units, 1024);
+    const dim3 grid(blocks < 512 ? blocks : 512);  // as many as run at once: each numbers the tokens first
+    if (p.f32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks);
+    else hipLaunchKernelGGL(prepare_kernel<bf16>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks);
     return check_launch("xent(prepare)");
   }
-  hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a);
+  hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a, p.amax_blocks);
   int rc = check_launch("xent(select)");
-  if (rc == DION_OK) rc = pack(x, d->dtype, st, "xent(pack hidden)");
-  if (rc == DION_OK && p.pack_w) rc = pack(w, d->dtype, st, "xent(pack weight)");
+  if (rc == DION_OK) rc = pack(x, tok, p, st, "xent(pack hidden)");
+  if (rc == DION_OK && p.wide) rc = pack(xg, tok, p, st, "xent(pack hidden for dW)");
+  if (rc == DION_OK && p.pack_w) rc = pack(w, tok, p, st, "xent(pack weight)");
   return rc;
 }
 
 // The W operand of a piece that starts at row v0: where it lies, or its limbs in the workspace (the
 // first piece's are there already).
-int piece_w(const DionXentDesc* d, const Plan& p, const void* weight, int v0, int n, char* ws, const uint16_t** w,
-            int64_t* ld, size_t* stride, hipStream_t st) {
+int piece_w(const DionXentDesc* d, const Plan& p, const void* weight, int v0, int n, const Tokens& tok, char* ws,
+            const uint16_t** w, int64_t* ld, size_t* stride, hipStream_t st) {
   if (!p.pack_w) {
     *w = static_cast<const uint16_t*>(weight) + static_cast<int64_t>(v0) * d->ld_weight;
     *ld = d->ld_weight;
@@ -448,7 +633,7 @@ int piece_w(const DionXentDesc* d, const Plan& p, const void* weight, int v0, in
   *w = reinterpret_cast<uint16_t*>(ws + p.wp);
   *ld = p.hidden_p;
   *stride = static_cast<size_t>(p.piece) * p.hidden_p;
-  return v0 == 0 ? DION_OK : pack(weight_args(d, p, weight, v0, n, ws), d->dtype, st, "xent(pack weight)");
+  return v0 == 0 ? DION_OK : pack(weight_args(d, p, weight, v0, n, ws), tok, p, st, "xent(pack weight)");
 }
 
 void logits_args(GemmArgs* a, const DionXentDesc* d, const Plan& p, const uint16_t* x, const uint16_t* w, int64_t ldw,
@@ -464,6 +649,7 @@ void logits_args(GemmArgs* a, const DionXentDesc* d, const Plan& p, const uint16
   a->splits = 1;
   a->tgt = tok.tgt;
   a->col0 = v0;
+  a->scale = p.f32 ? tok.scale + kScaleZ : nullptr;
 }
 
 int forward(const DionXentDesc* d, const void* hidden, const void* weight, const int64_t* target, float* loss,
@@ -479,14 +665,14 @@ int forward(const DionXentDesc* d, const void* hidden, const void* weight, const
     const uint16_t* w;
     int64_t ldw;
     size_t stride;
-    rc = piece_w(d, p, weight, v0, n, ws, &w, &ldw, &stride, st);
+    rc = piece_w(d, p, weight, v0, n, tok, ws, &w, &ldw, &stride, st);
     if (rc != DION_OK) return rc;
     GemmArgs a;
     logits_args(&a, d, p, x, w, ldw, stride, v0, n, tok);
     a.part = part;
     a.ldpart = p.tokens_p;
     a.tlogit = tok.tlogit;
-    rc = launch<false, false, EPI_STATS>(p.logits, a, d->tokens, n, st, "xent(logits)");
+    rc = launch<false, false, EPI_STATS>(p.f32, p.logits, a, d->tokens, n, st, "xent(logits)");
     if (rc != DION_OK) return rc;
   }
   // tiles that exist, the last piece's ragged one among them
@@ -518,20 +704,24 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     const uint16_t* w;
     int64_t ldw;
     size_t stride;
-    rc = piece_w(d, p, weight, v0, n, ws, &w, &ldw, &stride, st);
+    rc = piece_w(d, p, weight, v0, n, tok, ws, &w, &ldw, &stride, st);
     if (rc != DION_OK) return rc;
     GemmArgs a;
     logits_args(&a, d, p, x, w, ldw, stride, v0, n, tok);
     a.lse = tok.lse;
     a.gl = tok.gl;
-    for (int l = 0; l < p.limbs_g; ++l) a.g[l] = g + l * gstride;
-    a.nlimb = p.limbs_g;
+    uint16_t* wide = p.f32 ? g : g + gstride;  // the fp16 limbs
+    if (!p.f32) a.gb = g;
+    if (p.wide) {
+      a.gh[0] = wide;
+      a.gh[1] = wide + gstride;
+    }
     a.ldg = p.piece;
-    rc = launch<false, false, EPI_GRAD>(p.logits, a, p.tokens_p, n, st, "xent(logit gradients)");
+    rc = launch<false, false, EPI_GRAD>(p.f32, p.logits, a, p.tokens_p, n, st, "xent(logit gradients)");
     if (rc != DION_OK) return rc;
     if (grad_hidden) {
       memset(&a, 0, sizeof(a));
-      segments(&a, g, gstride, d->dtype == DION_DTYPE_F32 ? 3 : 1, w, stride, p.limbs_in);
+      segments(&a, g, gstride, p.limbs_in, w, stride, p.limbs_in);
       a.ldr = p.piece;
       a.ldc = ldw;
       a.cols = p.pack_w ? p.hidden_p : d->hidden;
@@ -543,12 +733,14 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.ldslab = p.hidden_p;
       a.slab_stride = static_cast<int64_t>(p.tokens_p) * p.hidden_p;
       a.add = v0 > 0;
-      rc = launch<false, true, EPI_SLAB>(p.dx, a, d->tokens, d->hidden, st, "xent(grad hidden)");
+      rc = launch<false, true, EPI_SLAB>(p.f32, p.dx, a, d->tokens, d->hidden, st, "xent(grad hidden)");
       if (rc != DION_OK) return rc;
     }
     if (grad_weight) {
       memset(&a, 0, sizeof(a));
-      segments(&a, g, gstride, p.limbs_g, x, xstride, p.limbs_in);
+      if (p.wide) segments(&a, wide, gstride, 2, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
+      else segments(&a, g, gstride, 1, x, xstride, 1);
+      a.scale = p.wide ? tok.scale + kScaleDw : nullptr;
       a.ldr = p.piece;
       a.ldc = p.hidden_p;
       a.cols = d->hidden;
@@ -563,7 +755,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.out_vec = d->hidden % 4 == 0 && d->ld_grad_weight % 4 == 0 && aligned16(grad_weight);
       // tiles stay inside the piece of g (a multiple of 256 words): what lies past n there makes rows
       // that are not stored
-      rc = launch<true, true, EPI_OUT>(p.dw, a, n, d->hidden, st, "xent(grad weight)");
+      rc = launch<true, true, EPI_OUT>(p.wide, pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2), a, n, d->hidden, st, "xent(grad weight)");
       if (rc != DION_OK) return rc;
     }
   }
@@ -571,13 +763,14 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     const long blocks = ceil_div(d->tokens * ceil_div(d->hidden, 4), 256);
     const dim3 grid(blocks < 8192 ? blocks : 8192);
     const int64_t sstride = static_cast<int64_t>(p.tokens_p) * p.hidden_p;
+    const float* scale = p.f32 ? tok.scale + kScaleDx : nullptr;
     if (d->dtype == DION_DTYPE_F32)
       hipLaunchKernelGGL(round_kernel<float>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden,
+                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl,
                          static_cast<float*>(grad_hidden), d->ld_grad_hidden);
     else
       hipLaunchKernelGGL(round_kernel<bf16>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden,
+                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl,
                          static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
     rc = check_launch("xent(round grad hidden)");
   }

@@ -38,9 +38,10 @@ def half_step(dtype):
 
 def xent(hidden, weight, target, ignore, grad_loss=None, total=None, start=0, out_dtype=None):
     """Loss, lse and gradients in 64 bits, and for each the largest error that the kernels' roundings
-    allow: fp32 sums of k terms in chains of 16 (k / 16 + 20 roundings of at most the sum of the terms'
-    magnitudes; three times as many for the limbs of fp32 inputs and what their products leave out), g
-    rounded to limbs, and one rounding of the result."""
+    allow.  Sums of k terms run in fp32 in chains of 16: k / 16 + 20 roundings of at most the sum of the
+    terms' magnitudes.  An operand of fp32 precision is two fp16 limbs: off by 2^-22 of each value and by
+    2^-39 of the largest, and a product of two such leaves out lo lo, 2^-22 again; its sum has three times
+    as many terms.  g is rounded to bf16 (2^-8), or to two limbs, and the result once."""
     f32 = hidden.dtype == torch.float32
     x, w = hidden.double(), weight.double()
     t, h = x.shape
@@ -50,8 +51,10 @@ def xent(hidden, weight, target, ignore, grad_loss=None, total=None, start=0, ou
         live = valid & (grad_loss != 0)
     x = torch.where(valid[:, None], x, torch.zeros_like(x))  # never read
     z = x @ w.t()
-    steps = lambda k: (k / 16 + 20) * (6 if f32 else 1) * U32  # noqa: E731
+    steps = lambda k: (k / 16 + 20) * (3 if f32 else 1) * U32 + (3 * 2.0 ** -22 if f32 else 0.0)  # noqa: E731
     ez = steps(h) * (x.abs() @ w.abs().t()).amax(1)  # of a logit of each token
+    if f32:
+        ez = ez + 2 * 2.0 ** -39 * h * x.abs().max() * w.abs().max()
     lse = torch.logsumexp(z, 1)
     at = (target - start).clamp(0, v - 1)
     here = valid & (target >= start) & (target < start + v)
@@ -70,17 +73,21 @@ def xent(hidden, weight, target, ignore, grad_loss=None, total=None, start=0, ou
     g = (p - onehot) * gl[:, None]
     rel_p = (ez + e_lse + 128 * U32)[:, None]
     x = torch.where(live[:, None], x, torch.zeros_like(x))
-    limbs = {1: 2.0 ** -8, 2: 2.0 ** -16, 3: 2.0 ** -24}
-    n_x = 3 if f32 else 1
-    n_w = 3 if f32 or out_dtype == torch.float32 else 1
+    wide = f32 or out_dtype == torch.float32
     # an error of p is at most rel_p of p; g's own rounding is relative to g
-    def bound(n, terms_of):
-        return terms_of(limbs[n] * g.abs() + (rel_p * p + 2 * U32) * gl.abs()[:, None])
+    e_p = (rel_p * p + 2 * U32) * gl.abs()[:, None]
+    e_x = (2.0 ** -22 if f32 else 2.0 ** -8) * g.abs() + e_p
+    e_w = (2.0 ** -22 if wide else 2.0 ** -8) * g.abs() + e_p
     r["grad_hidden"] = g @ w
-    r["e_grad_hidden"] = (bound(n_x, lambda e: e @ w.abs()) + steps(v) * (g.abs() @ w.abs())
+    tiny = 2.0 ** -148  # the spacing of fp32's least numbers, twice
+    floor_w = 2.0 ** -39 * w.abs().max() * g.abs().sum(1, keepdim=True) if f32 else 0.0
+    r["e_grad_hidden"] = (e_x @ w.abs() + steps(v) * (g.abs() @ w.abs()) + floor_w + tiny
                           + half_step(hidden.dtype) * r["grad_hidden"].abs())
     r["grad_weight"] = g.t() @ x
     od = out_dtype or weight.dtype
-    r["e_grad_weight"] = (bound(n_w, lambda e: e.t() @ x.abs()) + steps(t) * (g.abs().t() @ x.abs())
-                          + half_step(od) * r["grad_weight"].abs())
+    # X goes in times the power of two below gl, its largest under 2^15
+    e2 = torch.where(gl != 0, 2.0 ** torch.floor(torch.log2(gl.abs().clamp_min(1e-300))), torch.ones_like(gl))[:, None]
+    floor_x = 2.0 ** -39 * (x.abs() * e2).max() * (g.abs() / e2).sum(0)[:, None] if wide and t else 0.0
+    r["e_grad_weight"] = (e_w.t() @ x.abs() + (steps(t) + (2 * (t / 16 + 20) * U32 if wide else 0.0)) * (g.abs().t() @ x.abs())
+                          + floor_x + tiny + half_step(od) * r["grad_weight"].abs())
     return r

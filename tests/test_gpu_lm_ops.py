@@ -403,6 +403,38 @@ def test_xent_in_pieces_of_256_words(dtype, out_dtype, tokens, hidden, vocab):
     _close(dw, ref["grad_weight"], ref["e_grad_weight"], "grad_weight")
 
 
+@pytest.mark.parametrize("tokens", [40, 2500])
+def test_xent_fp32_over_many_magnitudes(tokens):
+    """Hidden states from 1e-12 to 1e3, weights from 1e-9, upstream gradients from 1e-20: the limbs' scales
+    follow the largest, and what a limb cannot hold is 2^-39 of it."""
+    x, w, t, gl = _xent_case(tokens, 64, 300, F32, 0.2)
+    g = torch.Generator().manual_seed(5)
+    x = x * 10.0 ** (torch.rand(tokens, 1, generator=g) * 15 - 12)
+    w = w * 10.0 ** (torch.rand(300, 1, generator=g) * 9 - 9)
+    gl = gl * 10.0 ** (-20 * torch.rand(tokens, generator=g))
+    for scale in (1.0, 1e-25, 1e12):
+        _xent_check(x * scale, w / scale, t, gl, out_dtype=F32)
+
+
+def test_xent_main_grad_in_fp32_precision():
+    """bf16 inputs and an fp32 grad_weight: off by no more of its 2-norm than a product in fp32 would be."""
+    x, w, t, gl = _xent_case(700, 256, 1500, BF16, 0.1)
+    ref = R.xent(x, w, t, -100, gl, out_dtype=F32)["grad_weight"]
+    a = (x.cuda(), w.cuda(), t.cuda())
+    _, lse = mda.linear_cross_entropy_forward(*a)
+    _, dw = mda.linear_cross_entropy_backward(gl.cuda(), *a, lse, grad_weight=torch.empty(1500, 256, device="cuda"))
+    assert float((dw.double().cpu() - ref).norm() / ref.norm()) < 1e-6
+
+
+def test_xent_infinity_stays_in_its_row_and_column():
+    x, w, t, gl = _xent_case(50, 64, 300, F32, 0.0)
+    clean = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    x[7, 5] = float("inf")
+    loss, lse = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    keep = torch.arange(50) != 7
+    assert not torch.isfinite(loss[7]) and torch.equal(loss[keep.cuda()], clean[0][keep.cuda()])
+
+
 def test_xent_is_bitwise_reproducible():
     x, w, t, gl = _xent_case(300, 128, 3000, BF16, 0.1)
     a = (x.cuda(), w.cuda(), t.cuda())
