@@ -74,13 +74,22 @@ def _empty(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _stream_of(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without a Stream object in between, where this torch has it: a microsecond of a small call's eight
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream_of)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def _call(fn, device: torch.device, *args) -> int:
     """`fn(*args, stream)` on the current stream of `device`, which need not be the current device."""
     index = device.index
-    if index == torch.cuda.current_device():
-        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if index == _device():
+        return fn(*args, _raw_stream(index))
     with torch.cuda.device(index):
-        return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        return fn(*args, _raw_stream(index))
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor:
