@@ -139,15 +139,11 @@ int dion_rms_norm_add(const DionNormDesc* d, const void* x, const void* residual
     a.sblock = d->scale_block;
     a.sblocks = static_cast<int>(ceil_div(d->cols, d->scale_block));
   }
-  const bool vec = d->cols % 8 == 0 && aligned16(x) && aligned16(weight) && d->ld_x % 8 == 0 && aligned16(y) &&
-                   d->ld_y % 8 == 0 &&
-                   (!residual || (aligned16(residual) && d->ld_residual % 8 == 0)) &&
-                   (!h || (aligned16(h) && d->ld_h % 8 == 0));
   const bool f32 = d->dtype == DION_DTYPE_F32;
-  if (!quant) return f32 ? rms::forward<float, Q8_NONE>(a, vec, stream) : rms::forward<bf16, Q8_NONE>(a, vec, stream);
-  const bool lanes = vec && a.sblock >= 8 && a.sblock <= 512 && (a.sblock & (a.sblock - 1)) == 0;
-  if (lanes) return f32 ? rms::forward<float, Q8_LANES>(a, vec, stream) : rms::forward<bf16, Q8_LANES>(a, vec, stream);
-  return f32 ? rms::forward<float, Q8_ANY>(a, vec, stream) : rms::forward<bf16, Q8_ANY>(a, vec, stream);
+  if (!quant) return f32 ? rms::forward<float, Q8_NONE>(a, stream) : rms::forward<bf16, Q8_NONE>(a, stream);
+  const bool lanes = a.sblock >= 8 && a.sblock <= 512 && (a.sblock & (a.sblock - 1)) == 0;
+  if (lanes) return f32 ? rms::forward<float, Q8_LANES>(a, stream) : rms::forward<bf16, Q8_LANES>(a, stream);
+  return f32 ? rms::forward<float, Q8_ANY>(a, stream) : rms::forward<bf16, Q8_ANY>(a, stream);
 }
 
 int dion_rms_norm_add_workspace_bytes(const DionNormDesc* d, size_t* bytes) {
@@ -192,12 +188,8 @@ int dion_rms_norm_add_backward(const DionNormDesc* d, const void* grad_y, const 
   a.ldgh = d->ld_grad_h;
   a.ldgx = d->ld_grad_x;
   a.ldgr = d->ld_grad_residual;
-  const bool vec = d->cols % 8 == 0 && aligned16(grad_y) && aligned16(h) && aligned16(weight) && d->ld_grad_y % 8 == 0 &&
-                   d->ld_h % 8 == 0 && (!grad_h || (aligned16(grad_h) && d->ld_grad_h % 8 == 0)) &&
-                   (!grad_x || (aligned16(grad_x) && d->ld_grad_x % 8 == 0)) &&
-                   (!grad_residual || (aligned16(grad_residual) && d->ld_grad_residual % 8 == 0));
-  if (d->dtype == DION_DTYPE_F32) return rms::backward<float>(a, vec, stream);
-  return rms::backward<bf16>(a, vec, stream);
+  if (d->dtype == DION_DTYPE_F32) return rms::backward<float>(a, stream);
+  return rms::backward<bf16>(a, stream);
 }
 
 int dion_xent_workspace_bytes(const DionXentDesc* d, int op, size_t* bytes) {

@@ -12,7 +12,7 @@ struct DropoutArgs {
   DropArgs drop;
 };
 
-// 16-byte accesses; grid y: rows; the ragged end of a row (cols % VEC) goes element by element
+// 16-byte accesses at any alignment; grid y: rows; the ragged end of a row (cols % VEC) goes element by element
 template <typename T, int VEC, bool RES>
 __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   const Key key = philox_key(a.drop);
@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
         float v[VEC], q[VEC];
         load_vec<VEC>(x + i * VEC, v);
         if constexpr (RES) load_vec<VEC>(r + i * VEC, q);
-        drop_vec<VEC>(v, static_cast<uint64_t>(row) * a.cols + i * VEC, key, a.drop);
+        drop_groups<VEC>(v, static_cast<uint64_t>(row) * a.cols + i * VEC, key, a.drop);
         if constexpr (RES) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) v[k] = __fadd_rn(v[k], q[k]);
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
       } else {
         for (int64_t c = nvec * VEC; c < a.cols; ++c) {
           float v = to_f32(x[c]);
-          drop_vec<1>(&v, static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
+          drop_one(&v, static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
           if constexpr (RES) v = __fadd_rn(v, to_f32(r[c]));
           o[c] = from_f32<T>(v);
         }
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256) dropout_vec_kernel(const DropoutArgs a) {
   }
 }
 
-// any strides: a thread makes the words of 4 consecutive elements and walks over row ends
+// rows that start within a group: a thread makes the words of 4 consecutive elements and walks over row ends
 template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_any_kernel(const DropoutArgs a) {
   const Key key = philox_key(a.drop);
@@ -80,9 +80,7 @@ int launch(DropoutArgs a, hipStream_t st) {
     a.rows = 1;
     a.ldx = a.ldr = a.ldo = a.cols;
   }
-  bool vec = aligned16(a.x) && aligned16(a.out) && (!RES || aligned16(a.residual));
-  // every row starts on a vector and on a group of 4 elements
-  if (a.rows > 1) vec = vec && a.cols % VEC == 0 && a.ldx % VEC == 0 && a.ldo % VEC == 0 && (!RES || a.ldr % VEC == 0);
+  const bool vec = a.rows == 1 || a.cols % 4 == 0;  // every row starts with a group of 4 elements
   constexpr long kBlocks = 256 * 16;  // 16 blocks of 256 threads for each of 256 CUs, then a loop
   if (vec) {
     const long bx = ceil_div(a.cols / VEC + 1, 256), by = a.rows < 32768 ? a.rows : 32768;

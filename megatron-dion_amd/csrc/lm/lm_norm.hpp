@@ -1,10 +1,11 @@
 // lm_norm.hpp -- residual RMS norm with dropout, 8-bit output, and its backward pass.
 //
-// One pass over the data: a row is held in registers (NV vectors of VEC elements for each of the
+// One pass over the data: a row is held in registers (NV vectors of 8 elements for each of the
 // LPR threads that share it) between its sum of squares and its scaling, so the forward reads x
 // and the residual and writes h and y once, and the backward reads gy, h and grad_h and writes the
 // gradients once.  Rows of up to 1024 elements go to a wave each (no barrier), longer ones to a
-// block.  VEC = 8 needs 16-byte aligned rows; VEC = 1 takes everything else.
+// block.  Rows may start and end anywhere: wide accesses need no alignment here, and only a row's last
+// vector goes element by element.
 
 struct NormArgs {
   const void *x, *residual, *weight, *gy, *gh;
@@ -20,10 +21,10 @@ struct NormArgs {
   int dropping;
 };
 
-template <int VEC>
+template <bool RAGGED>
 __device__ __forceinline__ void load_weight(const NormArgs& a, int c, float* w) {
-  if (a.w_bf16) load_vec<VEC>(static_cast<const bf16*>(a.weight) + c, w);
-  else load_vec<VEC>(static_cast<const float*>(a.weight) + c, w);
+  if (a.w_bf16) load8<RAGGED>(static_cast<const bf16*>(a.weight), c, a.cols, w);
+  else load8<RAGGED>(static_cast<const float*>(a.weight), c, a.cols, w);
 }
 
 // sum over the LPR threads that share a row; `red`: LPR / 64 floats of LDS (LPR > 64)
@@ -46,12 +47,13 @@ __device__ __forceinline__ float e4m3_clamp(float v) {  // NaN stays NaN
   return v > 448.0f ? 448.0f : v < -448.0f ? -448.0f : v;
 }
 
-// round_e4m3(v inv), VEC bytes
-template <int VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* y, const float* v, float inv) {
-  if constexpr (VEC == 1) {
-    *y = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[0] * inv), 0.0f, 0, false) & 0xFF);
-  } else {
+__device__ __forceinline__ uint8_t to_e4m3(float v) {
+  return static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v), 0.0f, 0, false) & 0xFF);
+}
+// round_e4m3(v inv) from column c of a row on
+template <bool RAGGED>
+__device__ __forceinline__ void store8_e4m3(uint8_t* row, int c, int cols, const float* v, float inv) {
+  if (!RAGGED || c + 8 <= cols) {
     u32x2 q;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -59,7 +61,11 @@ __device__ __forceinline__ void store_e4m3(uint8_t* y, const float* v, float inv
       w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(v[4 * k + 2] * inv), e4m3_clamp(v[4 * k + 3] * inv), w, true);
       q[k] = static_cast<uint32_t>(w);
     }
-    *reinterpret_cast<u32x2*>(y) = q;
+    *reinterpret_cast<u32x2_any*>(row + c) = q;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < cols) row[c + k] = to_e4m3(v[k] * inv);
   }
 }
 
@@ -70,7 +76,7 @@ enum { Q8_NONE = 0, Q8_LANES = 1, Q8_ANY = 2 };
 template <int LPR>
 constexpr int norm_threads() { return LPR > 64 ? LPR : 256; }
 
-template <typename T, int VEC, int LPR, int NV, int Q8>
+template <typename T, int LPR, int NV, int Q8, bool RAGGED>
 __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const NormArgs a) {
   constexpr int RPB = LPR > 64 ? 1 : 4;
   __shared__ float red[16];
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
   const int sub = LPR > 64 ? 0 : (threadIdx.x >> 6);
   const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + sub;
   const bool live = row < a.rows;  // whole waves: RPB == 4 has a row for each wave
-  float v[NV][VEC];
+  float v[NV][8];
   if constexpr (Q8 == Q8_ANY) {
     for (int i = t; i < a.sblocks; i += LPR) amax[sub * a.sblocks + i] = 0u;
     __syncthreads();
@@ -91,36 +97,36 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
     T* h = static_cast<T*>(a.h) + row * a.ldh;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
-      if (c < a.cols) load_vec<VEC>(x + c, v[i]);
+      const int c = (i * LPR + t) * 8;
+      if (c < a.cols) load8<RAGGED>(x, c, a.cols, v[i]);
     }
-    float q[NV][VEC];
+    float q[NV][8];
     if (a.residual) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
-        if (c < a.cols) load_vec<VEC>(r + c, q[i]);
+        const int c = (i * LPR + t) * 8;
+        if (c < a.cols) load8<RAGGED>(r, c, a.cols, q[i]);
       }
     }
     if (a.dropping) {
       const Key key = philox_key(a.drop);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
-        if (c < a.cols) drop_vec<VEC>(v[i], static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
+        const int c = (i * LPR + t) * 8;
+        if (c < a.cols) drop8<RAGGED>(v[i], static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
+      const int c = (i * LPR + t) * 8;
       if (c < a.cols) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
+        for (int k = 0; k < 8; ++k) {
           if (a.residual) v[i][k] = __fadd_rn(v[i][k], q[i][k]);
           v[i][k] = to_f32(from_f32<T>(v[i][k]));  // the norm is of h as it is stored
           ss = fmaf(v[i][k], v[i][k], ss);
         }
-        if (a.h) store_vec<VEC>(h + c, v[i]);
+        if (a.h) store8<RAGGED>(h, c, a.cols, v[i]);
       }
     }
   }
@@ -130,13 +136,13 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
   if (live) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
+      const int c = (i * LPR + t) * 8;
       if (c < a.cols) {
-        float w[VEC];
-        load_weight<VEC>(a, c, w);
+        float w[8];
+        load_weight<RAGGED>(a, c, w);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[i][k] = v[i][k] * rstd * w[k];
-        if constexpr (Q8 == Q8_NONE) store_vec<VEC>(static_cast<T*>(a.y) + row * a.ldy + c, v[i]);
+        for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] * rstd * w[k];
+        if constexpr (Q8 == Q8_NONE) store8<RAGGED>(static_cast<T*>(a.y) + row * a.ldy, c, a.cols, v[i]);
       }
     }
   }
@@ -146,17 +152,17 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
+        const int c = (i * LPR + t) * 8;
         float m = 0.0f;
         if (c < a.cols) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) m = fmaxf(m, fabsf(v[i][k]));  // passes over NaN
+          for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(v[i][k]));  // passes over NaN
         }
         for (int o = 1; o < span; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
         const float s = fmaxf(m / 448.0f, 1.17549435e-38f), inv = 1.0f / s;
         if (c < a.cols) {
           if ((t & (span - 1)) == 0) a.scale[row * a.sblocks + (c >> shift)] = s;
-          store_e4m3<VEC>(static_cast<uint8_t*>(a.y) + row * a.ldy + c, v[i], inv);
+          store8_e4m3<RAGGED>(static_cast<uint8_t*>(a.y) + row * a.ldy, c, a.cols, v[i], inv);
         }
       }
     }
@@ -166,12 +172,12 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
+        const int c = (i * LPR + t) * 8;
         if (c < a.cols) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
+          for (int k = 0; k < 8; ++k) {
             const float y = fabsf(v[i][k]);
-            if (y == y) atomicMax(&amax[sub * a.sblocks + (c + k) / a.sblock], __float_as_uint(y));
+            if ((!RAGGED || c + k < a.cols) && y == y) atomicMax(&amax[sub * a.sblocks + (c + k) / a.sblock], __float_as_uint(y));
           }
         }
       }
@@ -183,13 +189,14 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
       uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.ldy;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
+        const int c = (i * LPR + t) * 8;
         if (c < a.cols) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const float s = fmaxf(__uint_as_float(amax[sub * a.sblocks + (c + k) / a.sblock]) / 448.0f, 1.17549435e-38f);
-            store_e4m3<1>(y + c + k, &v[i][k], 1.0f / s);
-          }
+          for (int k = 0; k < 8; ++k)
+            if (!RAGGED || c + k < a.cols) {
+              const float s = fmaxf(__uint_as_float(amax[sub * a.sblocks + (c + k) / a.sblock]) / 448.0f, 1.17549435e-38f);
+              y[c + k] = to_e4m3(v[i][k] * (1.0f / s));
+            }
         }
       }
     }
@@ -197,41 +204,41 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
 }
 
 // Weight-gradient partials: each block (or wave, LPR == 64) sums its rows in registers.
-template <typename T, int VEC, int LPR, int NV>
+template <typename T, int LPR, int NV, bool RAGGED>
 __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const NormArgs a) {
   constexpr int RPB = LPR > 64 ? 1 : 4;
   __shared__ float red[16];
   const int t = LPR > 64 ? threadIdx.x : (threadIdx.x & 63);
   const int64_t first = LPR > 64 ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   const int64_t step = static_cast<int64_t>(gridDim.x) * RPB;
-  float w[NV][VEC], dw[NV][VEC];
+  float w[NV][8], dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * LPR + t) * VEC;
+    const int c = (i * LPR + t) * 8;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) w[i][k] = dw[i][k] = 0.0f;
-    if (c < a.cols) load_weight<VEC>(a, c, w[i]);
+    for (int k = 0; k < 8; ++k) w[i][k] = dw[i][k] = 0.0f;
+    if (c < a.cols) load_weight<RAGGED>(a, c, w[i]);
   }
   Key key = {0, 0, 0, 0};
   if (a.dropping) key = philox_key(a.drop);
   for (int64_t row = first; row < a.rows; row += step) {
     const float rstd = a.rstd[row];
-    float u[NV][VEC], g[NV][VEC], q[NV][VEC], dot = 0.0f;  // u = h rstd, g = gy then w gy
+    float u[NV][8], g[NV][8], q[NV][8], dot = 0.0f;  // u = h rstd, g = gy then w gy
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
+      const int c = (i * LPR + t) * 8;
       if (c < a.cols) {
-        load_vec<VEC>(static_cast<const T*>(a.h_in) + row * a.ldh + c, u[i]);
-        load_vec<VEC>(static_cast<const T*>(a.gy) + row * a.ldgy + c, g[i]);
-        if (a.gh) load_vec<VEC>(static_cast<const T*>(a.gh) + row * a.ldgh + c, q[i]);
+        load8<RAGGED>(static_cast<const T*>(a.h_in) + row * a.ldh, c, a.cols, u[i]);
+        load8<RAGGED>(static_cast<const T*>(a.gy) + row * a.ldgy, c, a.cols, g[i]);
+        if (a.gh) load8<RAGGED>(static_cast<const T*>(a.gh) + row * a.ldgh, c, a.cols, q[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
+      const int c = (i * LPR + t) * 8;
       if (c < a.cols) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
+        for (int k = 0; k < 8; ++k) {
           u[i][k] *= rstd;
           dw[i][k] = fmaf(g[i][k], u[i][k], dw[i][k]);
           g[i][k] *= w[i][k];
@@ -243,19 +250,19 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const Nor
       const float mean = row_sum<LPR>(dot, red) / static_cast<float>(a.cols);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LPR + t) * VEC;
+        const int c = (i * LPR + t) * 8;
         if (c < a.cols) {
-          float d[VEC];
+          float d[8];
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) d[k] = rstd * (g[i][k] - u[i][k] * mean);
+          for (int k = 0; k < 8; ++k) d[k] = rstd * (g[i][k] - u[i][k] * mean);
           if (a.gh) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) d[k] += q[i][k];
+            for (int k = 0; k < 8; ++k) d[k] += q[i][k];
           }
-          if (a.gr) store_vec<VEC>(static_cast<T*>(a.gr) + row * a.ldgr + c, d);
+          if (a.gr) store8<RAGGED>(static_cast<T*>(a.gr) + row * a.ldgr, c, a.cols, d);
           if (a.gx) {
-            if (a.dropping) drop_vec<VEC>(d, static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
-            store_vec<VEC>(static_cast<T*>(a.gx) + row * a.ldgx + c, d);
+            if (a.dropping) drop8<RAGGED>(d, static_cast<uint64_t>(row) * a.cols + c, key, a.drop);
+            store8<RAGGED>(static_cast<T*>(a.gx) + row * a.ldgx, c, a.cols, d);
           }
         }
       }
@@ -265,8 +272,8 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_bwd_kernel(const Nor
     float* p = a.part + first * a.cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LPR + t) * VEC;
-      if (c < a.cols) store_vec<VEC>(p + c, dw[i]);
+      const int c = (i * LPR + t) * 8;
+      if (c < a.cols) store8<RAGGED>(p, c, a.cols, dw[i]);
     }
   }
 }
@@ -313,59 +320,48 @@ long bwd_blocks(int64_t rows, bool wave_rows) {
   const long want = wave_rows ? ceil_div(rows, 4) : rows;
   return want < 1024 ? (want < 1 ? 1 : want) : 1024;
 }
-bool wave_rows(int cols, bool vec) { return vec ? cols <= 1024 : cols <= 512; }
+bool wave_rows(int cols) { return cols <= 1024; }
 
-size_t ws_bytes(const DionNormDesc* d) {  // the larger of the two layouts: alignment is not known here
-  const long a = bwd_blocks(d->rows, true) * 4, b = bwd_blocks(d->rows, false);
-  return sizeof(float) * static_cast<size_t>(a > b ? a : b) * d->cols;
+size_t ws_bytes(const DionNormDesc* d) {
+  const bool w = wave_rows(d->cols);
+  return sizeof(float) * static_cast<size_t>(bwd_blocks(d->rows, w)) * (w ? 4 : 1) * d->cols;
+}
+
+// The threads of a row: a wave for up to 1024 columns, else as many as hold it in two vectors each.
+// f(LPR, NV)
+template <typename F>
+void with_row(int cols, F&& f) {
+  using std::integral_constant;
+  if (cols <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+  else if (cols <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (cols <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (cols <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  else if (cols <= 8192) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
 
 template <typename T, int Q8>
-int forward(const NormArgs& a, bool vec, hipStream_t st) {
-#define DION_NORM_FWD(VEC, LPR, NV)                                                                            \
-  do {                                                                                                         \
-    constexpr int RPB = LPR > 64 ? 1 : 4;                                                                      \
-    const size_t lds = Q8 == Q8_ANY ? sizeof(uint32_t) * RPB * a.sblocks : 0;                                         \
-    hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, LPR, NV, Q8>), dim3(ceil_div(a.rows, RPB)),                 \
-                       dim3(norm_threads<LPR>()), lds, st, a);                                                 \
-  } while (0)
-  if (vec) {
-    if (a.cols <= 512) DION_NORM_FWD(8, 64, 1);
-    else if (a.cols <= 1024) DION_NORM_FWD(8, 64, 2);
-    else if (a.cols <= 2048) DION_NORM_FWD(8, 256, 1);
-    else if (a.cols <= 4096) DION_NORM_FWD(8, 256, 2);
-    else if (a.cols <= 8192) DION_NORM_FWD(8, 512, 2);
-    else DION_NORM_FWD(8, 1024, 2);
-  } else if constexpr (Q8 != Q8_LANES) {
-    if (a.cols <= 512) DION_NORM_FWD(1, 64, 8);
-    else if (a.cols <= 1024) DION_NORM_FWD(1, 256, 4);
-    else if (a.cols <= 4096) DION_NORM_FWD(1, 256, 16);
-    else DION_NORM_FWD(1, 1024, 16);
-  }
-#undef DION_NORM_FWD
+int forward(const NormArgs& a, hipStream_t st) {
+  with_row(a.cols, [&](auto lpr, auto nv) {
+    constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, RPB = LPR > 64 ? 1 : 4;
+    const size_t lds = Q8 == Q8_ANY ? sizeof(uint32_t) * RPB * a.sblocks : 0;
+    const dim3 grid(ceil_div(a.rows, RPB)), block(norm_threads<LPR>());
+    if (a.cols % 8) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, Q8, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, Q8, false>), grid, block, lds, st, a);
+  });
   return check_launch("rms_norm_add");
 }
 
 template <typename T>
-int backward(const NormArgs& a, bool vec, hipStream_t st) {
-  const bool wr = wave_rows(a.cols, vec);
+int backward(const NormArgs& a, hipStream_t st) {
+  const bool wr = wave_rows(a.cols);
   const long blocks = bwd_blocks(a.rows, wr);
-#define DION_NORM_BWD(VEC, LPR, NV)                                                                         \
-  hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, LPR, NV>), dim3(blocks), dim3(norm_threads<LPR>()), 0, st, a)
-  if (vec) {
-    if (a.cols <= 512) DION_NORM_BWD(8, 64, 1);
-    else if (a.cols <= 1024) DION_NORM_BWD(8, 64, 2);
-    else if (a.cols <= 2048) DION_NORM_BWD(8, 256, 1);
-    else if (a.cols <= 4096) DION_NORM_BWD(8, 256, 2);
-    else if (a.cols <= 8192) DION_NORM_BWD(8, 512, 2);
-    else DION_NORM_BWD(8, 1024, 2);
-  } else {
-    if (a.cols <= 512) DION_NORM_BWD(1, 64, 8);
-    else if (a.cols <= 1024) DION_NORM_BWD(1, 256, 4);
-    else if (a.cols <= 4096) DION_NORM_BWD(1, 256, 16);
-    else DION_NORM_BWD(1, 1024, 16);
-  }
-#undef DION_NORM_BWD
+  with_row(a.cols, [&](auto lpr, auto nv) {
+    constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value;
+    const dim3 grid(blocks), block(norm_threads<LPR>());
+    if (a.cols % 8) hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, NV, false>), grid, block, 0, st, a);
+  });
   int rc = check_launch("rms_norm_add_backward");
   if (rc != DION_OK || a.gw == nullptr) return rc;
   hipLaunchKernelGGL(norm_dw_kernel, dim3(ceil_div(a.cols, 16)), dim3(1024), 0, st, a,

@@ -10,7 +10,8 @@
 // holds is never read.
 //
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
-// whose own rounding is as large, and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
+// whose own rounding is as large (two for dW of up to 256 tokens, where few roundings do not average out
+// and the second limb is free: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
 // an fp32 main_grad (three bf16 limbs measured 1.15 times the time of the whole pass, two left 2.6e-6 of
 // the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
 // limbs themselves.  The power of two that brings such an operand into fp16's range comes from its
@@ -27,6 +28,7 @@ struct Tokens {  // compact arrays, by the number a token has among those that t
   float* lse;    // [tokens_p] (backward)
   float* gl;     // [tokens_p] (backward)
   float* tlogit; // [tokens_p] (forward)
+  float* delta;  // [tokens_p] (backward, bf16 inputs): what the target's g lost when it was rounded
   float* amax;   // [3][kAmaxBlocks]: largest |X|, |W|, |X| 2^e of a block's share
   float* scale;  // [4]: kScaleZ ...
 };
@@ -81,6 +83,7 @@ __device__ __forceinline__ void put_token(const SelectArgs& a, int t, int n) {
   a.out.tgt[n] = known && y >= a.start && y < a.start + a.vocab ? static_cast<int>(y - a.start) : -1;
   if (a.gl) {
     a.out.gl[n] = known ? a.gl[t] : NAN;
+    a.out.delta[n] = 0.0f;
     a.out.lse[n] = a.lse[t];
   } else {
     a.out.tlogit[n] = known ? 0.0f : NAN;
@@ -95,7 +98,7 @@ struct PackArgs {
   int rows, cols;      // source extents
   int rows_p, cols_p;  // packed extents, zeros outside the source
   uint16_t* dst;       // limbs one after the other
-  int nlimb, vec;
+  int nlimb;
   int f16;             // fp16 limbs of the values times `mul` (a parameter), else one bf16
   int amax;            // f16: which row of Tokens::amax
   const float* gl;     // not NULL: times the power of two below |gl| of the row's token, too
@@ -128,7 +131,7 @@ __device__ __forceinline__ float block_amax(const float* p, int n) {
 struct AmaxArgs {
   const void *x, *w;
   int64_t ldx, ldw;
-  int tokens, vocab, hidden, vecx, vecw;
+  int tokens, vocab, hidden;
   int want_x, want_w, want_xg;
   const int64_t* target;
   const float* gl;
@@ -137,14 +140,9 @@ struct AmaxArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ float amax8(const T* p, int c, int cols, int vec) {
+__device__ __forceinline__ float amax8(const T* p, int c, int cols) {
   float v[8], m = 0.0f;
-  if (vec && c + 8 <= cols) {
-    load_vec<8>(p + c, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_f32(p[c + k]) : 0.0f;
-  }
+  load8(p, c, cols, v);
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float y = fabsf(v[k]);
@@ -164,14 +162,14 @@ __global__ void __launch_bounds__(256) amax_kernel(const AmaxArgs a) {
     for (int64_t i = first; i < static_cast<int64_t>(a.tokens) * per; i += step) {
       const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
       if (a.target[t] == a.ignore || (a.gl && a.gl[t] == 0.0f)) continue;
-      const float m = amax8(static_cast<const T*>(a.x) + t * a.ldx, c, a.hidden, a.vecx);
+      const float m = amax8(static_cast<const T*>(a.x) + t * a.ldx, c, a.hidden);
       mx = fmaxf(mx, m);
       if (a.want_xg) mg = fmaxf(mg, m * pow2_below(a.gl[t]));
     }
   if (a.want_w)
     for (int64_t i = first; i < static_cast<int64_t>(a.vocab) * per; i += step) {
       const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
-      mw = fmaxf(mw, amax8(static_cast<const T*>(a.w) + t * a.ldw, c, a.hidden, a.vecw));
+      mw = fmaxf(mw, amax8(static_cast<const T*>(a.w) + t * a.ldw, c, a.hidden));
     }
   float v[3] = {mx, mw, mg <= 3.402823466e38f ? mg : 3.402823466e38f};
 #pragma unroll
@@ -194,14 +192,8 @@ __device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, co
 #pragma unroll
   for (int k = 0; k < 8; ++k) v[k] = 0.0f;
   if (row < rows) {
-    const T* s = static_cast<const T*>(a.src) + static_cast<int64_t>(index ? index[row] : row) * a.ld + c;
-    if (a.vec && c + 8 <= a.cols) {
-      load_vec<8>(s, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < a.cols) v[k] = to_f32(s[k]);
-    }
+    const T* s = static_cast<const T*>(a.src) + static_cast<int64_t>(index ? index[row] : row) * a.ld;
+    if (c < a.cols) load8(s, c, a.cols, v);
   }
   uint16_t* o = a.dst + static_cast<int64_t>(row) * a.cols_p + c;
   u32x4 q;
@@ -325,11 +317,14 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int parts
   }
 }
 
-// grad_hidden = the sum of the splits' slabs, rounded; zeros where a token takes no part
+// grad_hidden = the sum of the splits' slabs, rounded; zeros where a token takes no part.  A row of dX is
+// mostly its target's, whose g is near -gl: what that one number lost as a bf16 (up to 2^-8 of the row) is
+// put back in fp32, from one row of W.
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(const float* slab, int splits, int64_t stride, int64_t ldslab,
                                                     const int* pos, int tokens, int cols, const float* scale,
-                                                    const float* gl, T* out, int64_t ldo) {
+                                                    const float* gl, const Tokens tok, const T* w, int64_t ldw,
+                                                    T* out, int64_t ldo) {
   const int per = static_cast<int>((cols + 3) / 4);
   const int64_t n = static_cast<int64_t>(tokens) * per;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
@@ -341,9 +336,11 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
         v += *reinterpret_cast<const f32x4*>(slab + s * stride + static_cast<int64_t>(p) * ldslab + c);
     if (p >= 0 && scale) v = v * *scale * pow2_below(gl[p]);  // one after the other: their product may underflow
     T* o = out + static_cast<int64_t>(t) * ldo + c;
+    const float lost = p >= 0 && w ? tok.delta[p] : 0.0f;
+    const T* wy = w && lost != 0.0f ? w + static_cast<int64_t>(tok.tgt[p]) * ldw + c : nullptr;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (c + k < cols) o[k] = from_f32<T>(v[k]);
+      if (c + k < cols) o[k] = from_f32<T>(wy ? fmaf(lost, to_f32(wy[k]), v[k]) : v[k]);
   }
 }
 
@@ -352,7 +349,8 @@ struct Plan {
   int f32;             // fp32 inputs
   int wide;            // backward: grad_weight in fp32 precision
   int limbs_in;        // of X and W
-  int g_arrays;        // backward: 16-bit arrays of g: bf16 (bf16 inputs), fp16 hi and lo (wide)
+  int pair;            // backward: dW from two bf16 limbs of g
+  int g_arrays;        // backward: 16-bit arrays of g: bf16 (bf16 inputs), fp16 hi and lo (wide) or bf16 lo (pair)
   int logits, dx;      // tiles of the products (kTiles); dW's goes by the piece
   int tokens_p, hidden_p;
   bool pack_w;
@@ -402,7 +400,8 @@ Plan make_plan(const DionXentDesc* d, int op) {
   p.f32 = d->dtype == DION_DTYPE_F32;
   p.wide = op == DION_XENT_BACKWARD && (p.f32 || d->gw_dtype == DION_DTYPE_F32);
   p.limbs_in = p.f32 ? 2 : 1;
-  p.g_arrays = p.f32 ? 2 : p.wide ? 3 : 1;
+  p.pair = op == DION_XENT_BACKWARD && !p.wide && d->tokens <= 256;
+  p.g_arrays = p.f32 || p.pair ? 2 : p.wide ? 3 : 1;
   p.logits = pick_tile(d->tokens, d->vocab, 1, 3);
   p.dx = pick_tile(d->tokens, d->hidden, ceil_div(d->vocab, 256), d->tokens >= 256 ? 3 : d->tokens > 64 ? 2 : 1);
   const int br = kTiles[p.logits].br > kTiles[p.dx].br ? kTiles[p.logits].br : kTiles[p.dx].br;
@@ -432,7 +431,7 @@ Plan make_plan(const DionXentDesc* d, int op) {
     return o;
   };
   const size_t tp = static_cast<size_t>(p.tokens_p);
-  p.tok = take(512 + 3 * kAmaxBlocks * sizeof(float) + 6 * tp * 4);
+  p.tok = take(512 + 3 * kAmaxBlocks * sizeof(float) + 7 * tp * 4);
   p.xp = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
   if (p.wide) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
   if (p.f32 || p.wide) {
@@ -513,6 +512,7 @@ Tokens tokens_at(char* ws, const Plan& p) {
   t.lse = reinterpret_cast<float*>(t.tgt + n);
   t.gl = t.lse + n;
   t.tlogit = t.gl + n;
+  t.delta = t.tlogit + n;
   return t;
 }
 
@@ -530,7 +530,6 @@ PackArgs pack_args(const void* src, int64_t ld, const int* index, const int* cou
   a.cols_p = cols_p;
   a.dst = dst;
   a.nlimb = nlimb;
-  a.vec = aligned16(src) && ld % 8 == 0;
   a.f16 = f16;
   a.amax = amax;
   a.gl = gl;
@@ -577,8 +576,6 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
     m.tokens = a.tokens;
     m.vocab = d->vocab;
     m.hidden = d->hidden;
-    m.vecx = aligned16(hidden) && d->ld_hidden % 8 == 0;
-    m.vecw = aligned16(weight) && d->ld_weight % 8 == 0;
     m.want_x = m.want_w = p.f32;
     m.want_xg = p.wide;
     m.target = target;
@@ -711,7 +708,11 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     a.lse = tok.lse;
     a.gl = tok.gl;
     uint16_t* wide = p.f32 ? g : g + gstride;  // the fp16 limbs
-    if (!p.f32) a.gb = g;
+    if (!p.f32) {
+      a.gb[0] = g;
+      a.delta = tok.delta;
+    }
+    if (p.pair) a.gb[1] = g + gstride;
     if (p.wide) {
       a.gh[0] = wide;
       a.gh[1] = wide + gstride;
@@ -739,7 +740,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     if (grad_weight) {
       memset(&a, 0, sizeof(a));
       if (p.wide) segments(&a, wide, gstride, 2, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
-      else segments(&a, g, gstride, 1, x, xstride, 1);
+      else segments(&a, g, gstride, p.pair ? 2 : 1, x, xstride, 1);
       a.scale = p.wide ? tok.scale + kScaleDw : nullptr;
       a.ldr = p.piece;
       a.ldc = p.hidden_p;
@@ -766,12 +767,12 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     const float* scale = p.f32 ? tok.scale + kScaleDx : nullptr;
     if (d->dtype == DION_DTYPE_F32)
       hipLaunchKernelGGL(round_kernel<float>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl,
-                         static_cast<float*>(grad_hidden), d->ld_grad_hidden);
+                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl, tok,
+                         static_cast<const float*>(nullptr), int64_t(0),                         static_cast<float*>(grad_hidden), d->ld_grad_hidden);
     else
       hipLaunchKernelGGL(round_kernel<bf16>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl,
-                         static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
+                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl, tok,
+                         static_cast<const bf16*>(weight), d->ld_weight,                         static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
     rc = check_launch("xent(round grad hidden)");
   }
   return rc;

@@ -325,6 +325,8 @@ def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, tar
     Vocabulary shards (tensor parallel): weight holds the rows from `vocab_start` on of a vocabulary of
     `vocab_size` words (rows past it are padding), `group` the ranks that share it; every rank passes the
     same hidden states and targets and gets the whole vocabulary's loss."""
+    if group is not None and vocab_size is None:
+        raise RuntimeError("[DION_BAD_VOCAB] a vocabulary in shards needs vocab_size, the words of all of them")
     d, nbytes = _xent_desc(_lm_lib.XENT_FORWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index)
     device = hidden.device
     target = target.contiguous()

@@ -426,6 +426,23 @@ def test_xent_main_grad_in_fp32_precision():
     assert float((dw.double().cpu() - ref).norm() / ref.norm()) < 1e-6
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 8, 40, 300])
+def test_xent_bf16_gradients_are_near_their_rounding(tokens):
+    """bf16 results lose little more than their own rounding to bf16, few tokens or many: dX because what a
+    target's g loses is put back, dW of up to 256 tokens because g has two limbs there.  Of more tokens' dW
+    the roundings of g, as large as the result's and independent of them, add half their square: sqrt(2),
+    and 1.5 leaves room for 300 tokens' scatter."""
+    for seed in range(3):
+        x, w, t, gl = _xent_case(tokens, 256, 1500, BF16, 0.0, seed=100 * seed + tokens)
+        ref = R.xent(x, w, t, -100, gl, out_dtype=BF16)
+        a = (x.cuda(), w.cuda(), t.cuda())
+        _, lse = mda.linear_cross_entropy_forward(*a)
+        got = mda.linear_cross_entropy_backward(gl.cuda(), *a, lse)
+        for g, k, most in ((got[0], "grad_hidden", 1.2), (got[1], "grad_weight", 1.2 if tokens <= 256 else 1.5)):
+            off = (g.double().cpu() - ref[k]).norm()
+            assert float(off) <= most * float((ref[k].to(BF16).double() - ref[k]).norm()), (k, seed)
+
+
 def test_xent_infinity_stays_in_its_row_and_column():
     x, w, t, gl = _xent_case(50, 64, 300, F32, 0.0)
     clean = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
@@ -485,6 +502,63 @@ def test_leading_axes_and_graph_capture():
             assert torch.equal(u, q), k
         seen.append(got[0])
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_two_captured_graphs_replayed_together():
+    """Large tiles and prepared batches in two graphs, each with its own memory, replayed on two streams."""
+    cases = [_xent_case(600, 64, 30000, BF16, 0.1, seed=3), _xent_case(40, 64, 3000, F32, 0.1, seed=4)]
+    dev = [tuple(u.cuda() for u in c) for c in cases]
+
+    def step(x, w, t, gl):
+        loss, lse = mda.linear_cross_entropy_forward(x, w, t)
+        return (loss, *mda.linear_cross_entropy_backward(gl, x, w, t, lse))
+
+    want = [step(*c) for c in dev]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in dev:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(*c))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for o in outs:
+            for u in o:
+                u.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, q in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, q))
+        step(*dev[0])  # eager work in between
+
+
+def test_xent_weight_past_31_bits_of_elements():
+    """530000 x 4096 words: offsets of over 2^31 elements in weight and grad_weight."""
+    tokens, hidden, vocab = 6, 4096, 530000
+    torch.manual_seed(0)
+    w = torch.empty(vocab, hidden, dtype=BF16, device="cuda").normal_(0, 0.02)
+    x = torch.randn(tokens, hidden, device="cuda").to(BF16)
+    t = torch.tensor([0, vocab - 1, vocab - 2, 525000, 262144, -100], device="cuda")
+    gl = torch.rand(tokens, device="cuda")
+    loss, lse = mda.linear_cross_entropy_forward(x, w, t)
+    z = torch.cat([x.float() @ w[k:k + 65536].float().t() for k in range(0, vocab, 65536)], 1).double()
+    ref = torch.logsumexp(z, 1)
+    live = t >= 0
+    want = torch.where(live, ref - z.gather(1, t.clamp_min(0)[:, None])[:, 0], torch.zeros_like(ref))
+    # logits of |x||w| sums of 4096 terms of 0.016 on average in fp32, twice
+    assert float((loss.double() - want).abs().max()) < 2 * (4096 / 16 + 20) * R.U32 * 66 + 1e-5
+    _, dw = mda.linear_cross_entropy_backward(gl, x, w, t, lse, need_hidden=False)
+    p = torch.exp(z - ref[:, None])
+    p[live.nonzero()[:, 0], t[live]] -= 1
+    p *= torch.where(live, gl, torch.zeros_like(gl))[:, None]
+    for k in (0, 262144, 524289, 525000, vocab - 2, vocab - 1):
+        row = (p[:, k] @ x.double())
+        tol = (2.0 ** -16 + 1e-4) * (p[:, k].abs() @ x.double().abs()) + 2.0 ** -8 * row.abs()
+        assert bool(((dw[k].double() - row).abs() <= tol).all()), k
 
 
 def test_two_streams_at_once():

@@ -163,6 +163,8 @@ def test_python_calls_refuse():
     assert lm_ops._rng(0.0, None, dev) is None
     r = lm_ops._rng(0.5, (-1, 1 << 64), dev)
     assert (r.seed, r.offset) == ((1 << 64) - 1, 0)
+    with pytest.raises(RuntimeError, match="DION_BAD_VOCAB"):
+        mda.linear_cross_entropy_forward(x, w, t, group=object())
     with pytest.raises(RuntimeError, match="DION_NO_MAIN_GRAD"):
         mda.linear_cross_entropy(x, w, t, into_main_grad=True)
     with pytest.raises(RuntimeError, match="DION_BAD_GRAD_OUT"):
