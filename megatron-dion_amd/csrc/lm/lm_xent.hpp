@@ -44,29 +44,40 @@ struct SelectArgs {
   Tokens out;
 };
 
-// Numbers the tokens that take part, in order; the whole block (1024 threads) takes part.
-// f(t, n): token t (this thread's) has the number n, -1: none.  Returns how many there are.
+// Numbers the tokens that take part, in order; the whole block (1024 threads) takes part, 4 tokens a
+// thread at a time.  f(t, n): token t (this thread's) has the number n, -1: none.  Returns how many there are.
 template <typename F>
 __device__ __forceinline__ int select(const SelectArgs& a, F&& f) {
   __shared__ int wsum[16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int t0 = 0; t0 < a.tokens; t0 += 1024) {
-    const int t = t0 + threadIdx.x;
-    bool in = false;
-    if (t < a.tokens) {
-      in = a.target[t] != a.ignore;
-      if (a.gl) in = in && !(a.gl[t] == 0.0f);  // NaN takes part
+  for (int t0 = 0; t0 < a.tokens; t0 += 4096) {
+    const int t = t0 + 4 * static_cast<int>(threadIdx.x);
+    bool in[4];
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      in[k] = t + k < a.tokens && a.target[t + k] != a.ignore && (!a.gl || !(a.gl[t + k] == 0.0f));  // NaN takes part
+      mine += in[k];
     }
-    const uint64_t mask = __ballot(in);
-    if (lane == 0) wsum[wave] = __popcll(mask);
+    int upto = mine;  // of the wave's lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int below = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += below;
+    }
+    if (lane == 63) wsum[wave] = upto;
     __syncthreads();
-    int before = base, all = 0;
+    int before = base + upto - mine, all = 0;
     for (int w = 0; w < 16; ++w) {
       if (w < wave) before += wsum[w];
       all += wsum[w];
     }
-    if (t < a.tokens) f(t, in ? before + __popcll(mask & ((1ull << lane) - 1)) : -1);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (t + k < a.tokens) f(t + k, in[k] ? before : -1);
+      before += in[k];
+    }
     base += all;
     __syncthreads();
   }
@@ -322,25 +333,35 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int parts
 // put back in fp32, from one row of W.
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(const float* slab, int splits, int64_t stride, int64_t ldslab,
-                                                    const int* pos, int tokens, int cols, const float* scale,
-                                                    const float* gl, const Tokens tok, const T* w, int64_t ldw,
-                                                    T* out, int64_t ldo) {
-  const int per = static_cast<int>((cols + 3) / 4);
+                                                    int tokens, int cols, const float* scale, const Tokens tok,
+                                                    const T* w, int64_t ldw, T* out, int64_t ldo) {
+  const int per = (cols + 7) / 8;
   const int64_t n = static_cast<int64_t>(tokens) * per;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 4;
-    const int p = pos[t];
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p >= 0)
-      for (int s = 0; s < splits; ++s)
-        v += *reinterpret_cast<const f32x4*>(slab + s * stride + static_cast<int64_t>(p) * ldslab + c);
-    if (p >= 0 && scale) v = v * *scale * pow2_below(gl[p]);  // one after the other: their product may underflow
-    T* o = out + static_cast<int64_t>(t) * ldo + c;
-    const float lost = p >= 0 && w ? tok.delta[p] : 0.0f;
-    const T* wy = w && lost != 0.0f ? w + static_cast<int64_t>(tok.tgt[p]) * ldw + c : nullptr;
+    const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
+    const int p = tok.pos[t];
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (p >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        float q[8];
+        load_vec<8>(slab + s * stride + static_cast<int64_t>(p) * ldslab + c, q);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c + k < cols) o[k] = from_f32<T>(wy ? fmaf(lost, to_f32(wy[k]), v[k]) : v[k]);
+        for (int k = 0; k < 8; ++k) v[k] += q[k];
+      }
+      if (scale) {  // one after the other: their product may underflow
+        const float u = *scale, e2 = pow2_below(tok.gl[p]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = v[k] * u * e2;
+      }
+      const float lost = w ? tok.delta[p] : 0.0f;
+      if (lost != 0.0f) {
+        float q[8];
+        load8(w + static_cast<int64_t>(tok.tgt[p]) * ldw, c, cols, q);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(lost, q[k], v[k]);
+      }
+    }
+    store8(out + static_cast<int64_t>(t) * ldo, c, cols, v);
   }
 }
 
@@ -761,18 +782,19 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     }
   }
   if (grad_hidden) {
-    const long blocks = ceil_div(d->tokens * ceil_div(d->hidden, 4), 256);
+    const long blocks = ceil_div(d->tokens * ceil_div(d->hidden, 8), 256);
     const dim3 grid(blocks < 8192 ? blocks : 8192);
     const int64_t sstride = static_cast<int64_t>(p.tokens_p) * p.hidden_p;
-    const float* scale = p.f32 ? tok.scale + kScaleDx : nullptr;
-    if (d->dtype == DION_DTYPE_F32)
+    if (p.f32)
       hipLaunchKernelGGL(round_kernel<float>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl, tok,
-                         static_cast<const float*>(nullptr), int64_t(0),                         static_cast<float*>(grad_hidden), d->ld_grad_hidden);
+                         static_cast<int64_t>(p.hidden_p), static_cast<int>(d->tokens), d->hidden,
+                         tok.scale + kScaleDx, tok, static_cast<const float*>(nullptr), int64_t(0),
+                         static_cast<float*>(grad_hidden), d->ld_grad_hidden);
     else
       hipLaunchKernelGGL(round_kernel<bf16>, grid, dim3(256), 0, st, slab, p.splits, sstride,
-                         static_cast<int64_t>(p.hidden_p), tok.pos, static_cast<int>(d->tokens), d->hidden, scale, tok.gl, tok,
-                         static_cast<const bf16*>(weight), d->ld_weight,                         static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
+                         static_cast<int64_t>(p.hidden_p), static_cast<int>(d->tokens), d->hidden,
+                         static_cast<const float*>(nullptr), tok, static_cast<const bf16*>(weight), d->ld_weight,
+                         static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
     rc = check_launch("xent(round grad hidden)");
   }
   return rc;
