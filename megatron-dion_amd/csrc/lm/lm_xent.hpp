@@ -10,8 +10,8 @@
 // holds is never read.
 //
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
-// whose own rounding is as large (two for dW of up to 256 tokens, where few roundings do not average out
-// and the second limb is free: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
+// whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, one
+// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
 // an fp32 main_grad (three bf16 limbs measured 1.15 times the time of the whole pass, two left 2.6e-6 of
 // the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
 // limbs themselves.  The power of two that brings such an operand into fp16's range comes from its
@@ -370,8 +370,8 @@ struct Plan {
   int f32;             // fp32 inputs
   int wide;            // backward: grad_weight in fp32 precision
   int limbs_in;        // of X and W
-  int pair;            // backward: dW from two bf16 limbs of g
-  int g_arrays;        // backward: 16-bit arrays of g: bf16 (bf16 inputs), fp16 hi and lo (wide) or bf16 lo (pair)
+  int dw_limbs;        // backward: fp16 limbs of g for dW, 0: its bf16
+  int g_arrays;        // backward: 16-bit arrays of g: the bf16 (bf16 inputs), then the limbs
   int logits, dx;      // tiles of the products (kTiles); dW's goes by the piece
   int tokens_p, hidden_p;
   bool pack_w;
@@ -421,8 +421,8 @@ Plan make_plan(const DionXentDesc* d, int op) {
   p.f32 = d->dtype == DION_DTYPE_F32;
   p.wide = op == DION_XENT_BACKWARD && (p.f32 || d->gw_dtype == DION_DTYPE_F32);
   p.limbs_in = p.f32 ? 2 : 1;
-  p.pair = op == DION_XENT_BACKWARD && !p.wide && d->tokens <= 256;
-  p.g_arrays = p.f32 || p.pair ? 2 : p.wide ? 3 : 1;
+  p.dw_limbs = p.wide ? 2 : op == DION_XENT_BACKWARD && d->tokens <= 256 ? 1 : 0;
+  p.g_arrays = (p.f32 ? 0 : 1) + p.dw_limbs;
   p.logits = pick_tile(d->tokens, d->vocab, 1, 3);
   p.dx = pick_tile(d->tokens, d->hidden, ceil_div(d->vocab, 256), d->tokens >= 256 ? 3 : d->tokens > 64 ? 2 : 1);
   const int br = kTiles[p.logits].br > kTiles[p.dx].br ? kTiles[p.logits].br : kTiles[p.dx].br;
@@ -454,8 +454,8 @@ Plan make_plan(const DionXentDesc* d, int op) {
   const size_t tp = static_cast<size_t>(p.tokens_p);
   p.tok = take(512 + 3 * kAmaxBlocks * sizeof(float) + 7 * tp * 4);
   p.xp = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
-  if (p.wide) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
-  if (p.f32 || p.wide) {
+  if (p.dw_limbs) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
+  if (p.f32 || p.dw_limbs) {
     const long units = (d->tokens + (p.f32 ? d->vocab : 0)) * ceil_div(d->hidden, 8);
     p.amax_blocks = static_cast<int>(units > kAmaxBlocks * 1024L ? kAmaxBlocks : ceil_div(units, 1024));
   }
@@ -598,7 +598,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
     m.vocab = d->vocab;
     m.hidden = d->hidden;
     m.want_x = m.want_w = p.f32;
-    m.want_xg = p.wide;
+    m.want_xg = p.dw_limbs > 0;
     m.target = target;
     m.gl = gl;
     m.ignore = d->ignore_index;
@@ -614,7 +614,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   memset(&xg, 0, sizeof(xg));
   memset(&w, 0, sizeof(w));
   xg.cols_p = w.cols_p = 8;
-  if (p.wide) {
+  if (p.dw_limbs) {
     xg = x;
     xg.dst = reinterpret_cast<uint16_t*>(ws + p.xg);
     xg.f16 = 1;
@@ -633,7 +633,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a, p.amax_blocks);
   int rc = check_launch("xent(select)");
   if (rc == DION_OK) rc = pack(x, tok, p, st, "xent(pack hidden)");
-  if (rc == DION_OK && p.wide) rc = pack(xg, tok, p, st, "xent(pack hidden for dW)");
+  if (rc == DION_OK && p.dw_limbs) rc = pack(xg, tok, p, st, "xent(pack hidden for dW)");
   if (rc == DION_OK && p.pack_w) rc = pack(w, tok, p, st, "xent(pack weight)");
   return rc;
 }
@@ -730,14 +730,10 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     a.gl = tok.gl;
     uint16_t* wide = p.f32 ? g : g + gstride;  // the fp16 limbs
     if (!p.f32) {
-      a.gb[0] = g;
+      a.gb = g;
       a.delta = tok.delta;
     }
-    if (p.pair) a.gb[1] = g + gstride;
-    if (p.wide) {
-      a.gh[0] = wide;
-      a.gh[1] = wide + gstride;
-    }
+    for (int l = 0; l < p.dw_limbs; ++l) a.gh[l] = wide + l * gstride;
     a.ldg = p.piece;
     rc = launch<false, false, EPI_GRAD>(p.f32, p.logits, a, p.tokens_p, n, st, "xent(logit gradients)");
     if (rc != DION_OK) return rc;
@@ -760,9 +756,9 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     }
     if (grad_weight) {
       memset(&a, 0, sizeof(a));
-      if (p.wide) segments(&a, wide, gstride, 2, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
-      else segments(&a, g, gstride, p.pair ? 2 : 1, x, xstride, 1);
-      a.scale = p.wide ? tok.scale + kScaleDw : nullptr;
+      if (p.dw_limbs) segments(&a, wide, gstride, p.dw_limbs, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
+      else segments(&a, g, gstride, 1, x, xstride, 1);
+      a.scale = p.dw_limbs ? tok.scale + kScaleDw : nullptr;
       a.ldr = p.piece;
       a.ldc = p.hidden_p;
       a.cols = d->hidden;
@@ -777,7 +773,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.out_vec = d->hidden % 4 == 0 && d->ld_grad_weight % 4 == 0 && aligned16(grad_weight);
       // tiles stay inside the piece of g (a multiple of 256 words): what lies past n there makes rows
       // that are not stored
-      rc = launch<true, true, EPI_OUT>(p.wide, pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2), a, n, d->hidden, st, "xent(grad weight)");
+      rc = launch<true, true, EPI_OUT>(p.dw_limbs > 0, pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2), a, n, d->hidden, st, "xent(grad weight)");
       if (rc != DION_OK) return rc;
     }
   }

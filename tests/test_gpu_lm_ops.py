@@ -426,19 +426,19 @@ def test_xent_main_grad_in_fp32_precision():
     assert float((dw.double().cpu() - ref).norm() / ref.norm()) < 1e-6
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 8, 40, 300])
+@pytest.mark.parametrize("tokens", [1, 3, 8, 40, 300, 600])
 def test_xent_bf16_gradients_are_near_their_rounding(tokens):
     """bf16 results lose little more than their own rounding to bf16, few tokens or many: dX because what a
-    target's g loses is put back, dW of up to 256 tokens because g has two limbs there.  Of more tokens' dW
-    the roundings of g, as large as the result's and independent of them, add half their square: sqrt(2),
-    and 1.5 leaves room for 300 tokens' scatter."""
+    target's g loses is put back, dW of up to 256 tokens because g is an fp16 there.  Of more tokens' dW the
+    roundings of g, as large as the result's and independent of them, add as much again: sqrt(2), and 1.6
+    leaves room for 300 tokens' scatter."""
     for seed in range(3):
         x, w, t, gl = _xent_case(tokens, 256, 1500, BF16, 0.0, seed=100 * seed + tokens)
         ref = R.xent(x, w, t, -100, gl, out_dtype=BF16)
         a = (x.cuda(), w.cuda(), t.cuda())
         _, lse = mda.linear_cross_entropy_forward(*a)
         got = mda.linear_cross_entropy_backward(gl.cuda(), *a, lse)
-        for g, k, most in ((got[0], "grad_hidden", 1.2), (got[1], "grad_weight", 1.2 if tokens <= 256 else 1.5)):
+        for g, k, most in ((got[0], "grad_hidden", 1.2), (got[1], "grad_weight", 1.2 if tokens <= 256 else 1.6)):
             off = (g.double().cpu() - ref[k]).norm()
             assert float(off) <= most * float((ref[k].to(BF16).double() - ref[k]).norm()), (k, seed)
 
@@ -557,7 +557,9 @@ def test_xent_weight_past_31_bits_of_elements():
     p *= torch.where(live, gl, torch.zeros_like(gl))[:, None]
     for k in (0, 262144, 524289, 525000, vocab - 2, vocab - 1):
         row = (p[:, k] @ x.double())
-        tol = (2.0 ** -16 + 1e-4) * (p[:, k].abs() @ x.double().abs()) + 2.0 ** -8 * row.abs()
+        # g is one fp16 here (2^-11 of it), p is off by the logits' 66 (4096 / 16 + 20) 2^-24 = 1.1e-3 at most
+        # and measured against fp32 logits, and the sum is rounded once
+        tol = (2.0 ** -11 + 1.1e-3) * (p[:, k].abs() @ x.double().abs()) + 2.0 ** -8 * row.abs()
         assert bool(((dw[k].double() - row).abs() <= tol).all()), k
 
 
