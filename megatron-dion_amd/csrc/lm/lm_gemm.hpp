@@ -72,8 +72,13 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // lane l's 16 bytes at base + voff land at LDS byte lds + 16 l.  Completion is counted by hand
 // (wait_barrier), which is why this is asm and not the builtin: with the builtin hipcc waits for
 // all of them before any LDS read.
+// ONCE: what is loaded is not loaded again by another block (non-temporal).
+template <bool ONCE>
 __device__ __forceinline__ void load_lds16(const i32x4& rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
+  else
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_barrier() {
@@ -91,7 +96,7 @@ __device__ __forceinline__ i32x4 make_rsrc(const void* p, uint32_t bytes) {
 
 // One operand's tile: BN rows (KC) or columns (KS) by 64 k, loaded by NW waves in units of 1 KiB.
 // KTAIL: the operand ends with k in memory; the other operand is zero there, but 0 x NaN is not.
-template <int BN, bool KS, int NW, bool KTAIL>
+template <int BN, bool KS, int NW, bool KTAIL, bool ONCE>
 struct Tile {
   static constexpr int kBytes = BN * kBK * 2;
   static constexpr int kUnits = kBytes / 1024;
@@ -136,7 +141,7 @@ struct Tile {
   __device__ __forceinline__ void issue(int wave, uint32_t lds) const {
     uint32_t v = voff[U];
     if constexpr (!KS && KTAIL) v = kk[U] < kleft ? v : kOob;
-    load_lds16(rsrc, v, lds + (wave * kPerWave + U) * 1024);
+    load_lds16<ONCE>(rsrc, v, lds + (wave * kPerWave + U) * 1024);
   }
 };
 
@@ -224,12 +229,13 @@ __device__ __forceinline__ float pow2_below(float x) {
 }
 constexpr float kGradScale = 8192.0f;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
 
-template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF>
+// ONCE: one tile of rows, so that every part of C is read by one block.
+template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF, bool ONCE>
 __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const GemmArgs a) {
   constexpr int NWR = BR / WR, NWC = BC / WC, NW = NWR * NWC;
   constexpr int TR = WR / 32, TC = WC / 32;
-  using RT = Tile<BR, RKS, NW, false>;
-  using CT = Tile<BC, CKS, NW, true>;
+  using RT = Tile<BR, RKS, NW, false, false>;
+  using CT = Tile<BC, CKS, NW, true, ONCE>;
   constexpr int kStage = RT::kBytes + CT::kBytes;
   constexpr int kLoads = RT::kPerWave + CT::kPerWave;
   extern __shared__ __align__(16) char lds[];

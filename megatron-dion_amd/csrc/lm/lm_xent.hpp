@@ -489,13 +489,13 @@ void segments(GemmArgs* a, const uint16_t* r, size_t rstride, int rlimbs, const 
       }
 }
 
-template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF>
+template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF, bool ONCE = false>
 int launch_tile(GemmArgs a, long rows, long cols, hipStream_t st, const char* what) {
   a.row_tiles = static_cast<int>(ceil_div(rows, BR));
   a.col_tiles = static_cast<int>(ceil_div(cols, BC));
   constexpr int threads = 64 * (BR / WR) * (BC / WC);
   constexpr size_t lds = static_cast<size_t>(NBUF) * (BR + BC) * kBK * 2;
-  auto* kernel = gemm_kernel<BR, BC, WR, WC, RKS, CKS, F16, EPI, NBUF>;
+  auto* kernel = gemm_kernel<BR, BC, WR, WC, RKS, CKS, F16, EPI, NBUF, ONCE>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
@@ -510,7 +510,13 @@ int launch_as(int tile, const GemmArgs& a, long rows, long cols, hipStream_t st,
   switch (tile) {
     case 3: return launch_tile<256, 256, 64, 128, RKS, CKS, F16, EPI, 2>(a, rows, cols, st, what);
     case 2: return launch_tile<128, 128, 64, 64, RKS, CKS, F16, EPI, 2>(a, rows, cols, st, what);
-    case 1: return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);
+    case 1:
+      // The loss of up to 64 tokens alone: W passes by once, non-temporal.  One token under 32000 words of
+      // 4096: 60.2 us against 64.5 where a gigabyte of other weights has been read since, 63.7 against 48.1
+      // where the last-level cache still holds W.  The backward pass reads W twice and keeps it.
+      if constexpr (EPI == EPI_STATS)
+        if (rows <= 64) return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3, true>(a, rows, cols, st, what);
+      return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);
     default: return launch_tile<64, 64, 32, 32, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);
   }
 }
