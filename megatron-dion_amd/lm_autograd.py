@@ -92,7 +92,7 @@ class _RmsNormAdd(torch.autograd.Function):
             gx = lm_ops.dropout_add_backward(g, p=ctx.p, rng=ctx.rng) if need_x and ctx.p > 0.0 else g
             return gx if need_x else None, None, g if need_r else None, None, None, None
         b = lm_ops.rms_norm_add_backward(_rows(grad_y), h, weight, rstd, _rows(grad_h), p=ctx.p, rng=ctx.rng,
-                                         need_input=need_x or need_r, need_weight=need_w)
+                                         need_input=need_x or need_r, need_weight=need_w, need_residual=need_r)
         return b.grad_x if need_x else None, b.grad_weight, b.grad_residual if need_r else None, None, None, None
 
 

@@ -226,11 +226,13 @@ def _grad_weight(weight: torch.Tensor, out: Optional[torch.Tensor], accumulate: 
 def rms_norm_add_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
                           grad_h: Optional[torch.Tensor] = None, *, p: float = 0.0, rng: Optional[Rng] = None,
                           grad_weight: Optional[torch.Tensor] = None, accumulate: bool = False,
-                          need_input: bool = True, need_weight: bool = True) -> RmsNormAddGrads:
+                          need_input: bool = True, need_weight: bool = True, need_residual: bool = True
+                          ) -> RmsNormAddGrads:
     """Gradients of `rms_norm_add_forward`; `grad_h` is what reaches h past the norm (the residual
     stream's gradient), `p` and `rng` are the forward's.  An 8-bit y passes `grad_y` (x's dtype) as if
     it had not been rounded.  `grad_weight` (fp32 or bf16, e.g. `weight.main_grad`) is written, or with
-    `accumulate` added to; without it a new tensor of weight's dtype is returned."""
+    `accumulate` added to; without it a new tensor of weight's dtype is returned.  `need_input` asks for
+    grad_x and, with `need_residual`, for grad_residual."""
     rows, cols, ld = _rows(h, "h")
     ld_gy = _like(grad_y, "grad_y", h)
     ld_gh = 0 if grad_h is None else _like(grad_h, "grad_h", h)
@@ -250,7 +252,7 @@ def rms_norm_add_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.T
                            ld_gy, ld_gh, cols, cols)
     if need_input:
         gx = _empty(h)
-        if r is not None:
+        if r is not None and need_residual:
             gr = _empty(h)
     if need_weight:
         ws = _workspace(nbytes, device)
@@ -261,7 +263,7 @@ def rms_norm_add_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.T
                0 if ws is None else nbytes if nbytes > 16 else 16)
     if rc:
         _lm_lib.check(rc, "dion_rms_norm_add_backward")
-    return RmsNormAddGrads(gx, gx if gr is None else gr, gw)
+    return RmsNormAddGrads(gx, gr if r is not None else gx if need_residual else None, gw)
 
 
 # ------------------------------------------------------------------------------- linear cross entropy

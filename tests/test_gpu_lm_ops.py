@@ -144,6 +144,9 @@ def test_norm_forward_and_backward(dtype, rows, cols):
         _close(b.grad_weight, gw, tol + R.half_step(wdt) * gw.abs(), "grad_weight")
         if p == 0.0:
             assert b.grad_x is b.grad_residual
+        only = mda.rms_norm_add_backward(gy.cuda(), f.h, w.cuda(), f.rstd, None if gh is None else gh.cuda(), p=p,
+                                         rng=(seed, offset) if p else None, need_weight=False, need_residual=False)
+        assert torch.equal(only.grad_x, b.grad_x) and only.grad_residual is None and only.grad_weight is None
         # added to an fp32 and to a bf16 main_grad
         for mdt in (F32, BF16):
             main = _randn(8, cols, dtype=mdt).cuda()
@@ -239,7 +242,9 @@ def _xent_check(x, w, t, gl, *, out_dtype=None, pad=0, **kw):
 @pytest.mark.parametrize("tokens,hidden,vocab", [
     (1, 8, 1), (1, 64, 2), (1, 768, 1000), (2, 40, 127), (31, 64, 128), (32, 72, 129), (33, 64, 257), (64, 128, 300),
     (65, 200, 513), (128, 64, 1000), (129, 136, 255), (200, 768, 520), (256, 64, 256), (257, 320, 1003),
-    (513, 96, 2001)])
+    (513, 96, 2001), (40, 1, 50), (40, 7, 50), (2500, 64, 300),
+    # every tile: 128 x 128 and 256 x 256 of the logits, 128 x 128 and 256 x 256 of dW
+    (300, 72, 20000), (300, 72, 33000), (700, 72, 50000)])
 def test_xent(dtype, out_dtype, tokens, hidden, vocab):
     x, w, t, gl = _xent_case(tokens, hidden, vocab, dtype, 0.2 if tokens > 2 else 0.0)
     _xent_check(x, w, t, gl, out_dtype=out_dtype)
