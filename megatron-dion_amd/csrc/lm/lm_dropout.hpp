@@ -2,7 +2,9 @@
 //
 // Bytes per bf16 element: 2 read (4 with a residual), 2 written; 10 Philox rounds make the words of
 // 4 elements (20 32x32->64-bit products and 40 exclusive ors, about 25 VALU cycles per element of
-// a lane), which is near what the streams leave: the generator has to overlap the loads.
+// a lane), which is near what the streams leave: the generator has to overlap the loads.  Measured on
+// 8192 x 14336 bf16: 104-108 us (4.4-4.5 TB/s; a copy of 4 GiB reaches 4.77).  4 elements share a counter
+// because Philox makes 4 words; 32 bits for each keep p exact to 2^-32.
 
 struct DropoutArgs {
   const void *x, *residual;

@@ -1,5 +1,10 @@
 // lm_xent.hpp -- the linear cross entropy: tokens that take part, limbs, the pieces of the vocabulary.
 //
+// What it reads, writes and computes (T tokens that take part, H, V words): T H + V H elements, three
+// products of 2 T H V operations for loss and gradients, and a fourth because the logits are not kept.
+// 8192 x 4096 x 128256 in bf16: 6.6 ms forward, 27.4 with the gradients (1.25 PFLOP/s, bound by power, see
+// lm_gemm.hpp); one token x 4096 x 32000: 59 us, bound by reading W (4.4 TB/s).
+//
 // forward   select, pack X [, pack W] -> logits tiles, each leaving (maximum, sum of exp) of its columns
 //           for each token -> join them: lse, loss
 // backward  select, pack X -> for each piece of the vocabulary: [pack W], logits again, g = the
@@ -12,8 +17,8 @@
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
 // whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, one
 // fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
-// an fp32 main_grad (three bf16 limbs measured 1.15 times the time of the whole pass, two left 2.6e-6 of
-// the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
+// an fp32 main_grad (4096 tokens x 768 x 50257: 1.87 ms a pass, 2.34 with three bf16 limbs; two bf16 limbs
+// left 2.6e-6 of the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
 // limbs themselves.  The power of two that brings such an operand into fp16's range comes from its
 // largest finite value; g's is known, |p - [v = y]| <= 1 times the mantissa of the token's gl, whose
 // power of two goes into X (for dW) or is put back at the end (for dX).
