@@ -79,13 +79,15 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // lane l's 16 bytes at base + voff land at LDS byte lds + 16 l.  Completion is counted by hand
 // (wait_barrier), which is why this is asm and not the builtin: with the builtin hipcc waits for
 // all of them before any LDS read.
+// The wait states cover a descriptor or m0 that the instruction before has written, also from a vector
+// register (5), which hipcc does not look for in front of asm.
 // ONCE: what is loaded is not loaded again by another block (non-temporal).
 template <bool ONCE>
 __device__ __forceinline__ void load_lds16(const i32x4& rsrc, uint32_t voff, uint32_t lds) {
   if constexpr (ONCE)
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
   else
-    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rsrc), "{m0}"(lds) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_barrier() {
@@ -213,11 +215,6 @@ __device__ __forceinline__ void each(F&& f) {
   }
 }
 
-// The loop over steps of 64 k is software-pipelined by hand.  A step is four phases of 16 k; in each,
-// a wave's MFMAs run on fragments in registers while it reads the next phase's from LDS.  The barrier
-// stands before the last phase: there every wave has its last fragments of this step's tile, so the
-// tile's buffer is free for the step NBUF on, whose loads are issued in between the phase's MFMAs, and
-// the next step's tile has arrived (vmcnt), whose first fragments the phase reads.
 template <bool F16>
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
   if constexpr (F16)
@@ -236,6 +233,12 @@ __device__ __forceinline__ float pow2_below(float x) {
 }
 constexpr float kGradScale = 8192.0f;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
 
+// The loop over steps of 64 k is software-pipelined by hand.  A step is four phases of 16 k; in each,
+// a wave's MFMAs run on fragments in registers while it reads the next phase's from LDS.  The barrier
+// stands before the last phase: there every wave has its last fragments of this step's tile, so the
+// tile's buffer is free for the step NBUF on, whose loads are issued in between the phase's MFMAs, and
+// the next step's tile has arrived (vmcnt), whose first fragments the phase reads.
+//
 // ONCE: one tile of rows, so that every part of C is read by one block.
 template <int BR, int BC, int WR, int WC, bool RKS, bool CKS, bool F16, int EPI, int NBUF, bool ONCE>
 __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const GemmArgs a) {
