@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(norm_threads<LPR>()) norm_fwd_kernel(const Nor
   extern __shared__ uint32_t amax[];  // Q8_ANY: sblocks words for each row of the block
   const int t = LPR > 64 ? threadIdx.x : (threadIdx.x & 63);
   const int sub = LPR > 64 ? 0 : (threadIdx.x >> 6);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + sub;
+  const int64_t row = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * RPB + sub;
   const bool live = row < a.rows;  // whole waves: RPB == 4 has a row for each wave
   float v[NV][8];
   if constexpr (Q8 == Q8_ANY) {
@@ -347,7 +347,9 @@ int forward(const NormArgs& a, hipStream_t st) {
   with_row(a.cols, [&](auto lpr, auto nv) {
     constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, RPB = LPR > 64 ? 1 : 4;
     const size_t lds = Q8 == Q8_ANY ? sizeof(uint32_t) * RPB * a.sblocks : 0;
-    const dim3 grid(ceil_div(a.rows, RPB)), block(norm_threads<LPR>());
+    // a grid's axis has to stay below 2^32 threads: 2^21 blocks of up to 1024, then rows of them
+    const long blocks = ceil_div(a.rows, RPB), bx = blocks < (1 << 21) ? blocks : 1 << 21;
+    const dim3 grid(bx, ceil_div(blocks, bx)), block(norm_threads<LPR>());
     if (a.cols % 8) hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, Q8, true>), grid, block, lds, st, a);
     else hipLaunchKernelGGL((norm_fwd_kernel<T, LPR, NV, Q8, false>), grid, block, lds, st, a);
   });

@@ -440,8 +440,10 @@ Plan make_plan(const DionXentDesc* d, int op) {
     const size_t most = d->piece_bytes > 0 ? static_cast<size_t>(d->piece_bytes) : kPieceBytes;
     piece = static_cast<long>(most / (static_cast<size_t>(p.g_arrays) * p.tokens_p * 2)) / 256 * 256;
     if (p.pack_w && piece > 32768) piece = 32768;
-  } else if (p.pack_w) {
-    piece = 32768;
+  } else {
+    // a grid's axis has to stay below 2^32 threads: 2^22 tiles at most, of 256 x 256 by 512
+    piece = (1L << 38) / p.tokens_p / 256 * 256;
+    if (p.pack_w && piece > 32768) piece = 32768;
   }
   if (piece < 256) piece = 256;
   if (piece > vocab_p) piece = vocab_p;

@@ -184,6 +184,22 @@ def test_norm_in_8_bits(dtype, rows, cols, block):
     assert (top[1:] == 448).all()  # the largest of each block takes the largest code
 
 
+@pytest.mark.parametrize("rows,cols", [((1 << 26) + 6, 8), ((1 << 21) + 3, 1032)])
+def test_norm_of_more_rows_than_one_axis_of_a_grid_holds(rows, cols):
+    """64 threads a row make 2^32 of the first; the second fills an axis of 2^21 blocks."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda").normal_(generator=g)
+    w = _randn(4, cols)
+    f = mda.rms_norm_add_forward(x, w.cuda(), eps=1e-5)
+    for part in (slice(0, 70), slice((1 << 23) - 35, (1 << 23) + 35), slice(rows - 70, rows)):
+        part = slice(min(part.start, rows - 70), min(part.stop, rows))
+        want = _norm_reference(x[part].cpu(), w, None, 0.0, 0, 0, 1e-5)
+        # cols squares added in fp32, a root, a quotient and two products: (cols + 8) half steps; then bf16's
+        off = (cols + 8) * R.U32
+        _close(f.rstd[part], want[2], off * want[2], "rstd")
+        _close(f.y[part], want[3], (off + 2.0 ** -8) * want[3].abs(), "y")
+
+
 def test_norm_rows_do_not_mix_and_nan_stays_in_its_row():
     x, w = _randn(1, 6, 1024, dtype=BF16), torch.ones(1024)
     x[2, 5], x[4, 7] = float("nan"), float("inf")
@@ -566,6 +582,22 @@ def test_xent_weight_past_31_bits_of_elements():
         # and measured against fp32 logits, and the sum is rounded once
         tol = (2.0 ** -11 + 1.1e-3) * (p[:, k].abs() @ x.double().abs()) + 2.0 ** -8 * row.abs()
         assert bool(((dw[k].double() - row).abs() <= tol).all()), k
+
+
+def test_xent_of_more_tiles_than_one_axis_of_a_grid_holds():
+    """2^22 tokens x 131072 words are 2^23 tiles of 512 threads: two launches."""
+    tokens, hidden, vocab = 1 << 22, 8, 131072
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty(tokens, hidden, dtype=BF16, device="cuda").normal_(generator=g)
+    w = torch.empty(vocab, hidden, dtype=BF16, device="cuda").normal_(generator=g)
+    t = torch.randint(0, vocab, (tokens,), generator=g, device="cuda")
+    loss, lse = mda.linear_cross_entropy_forward(x, w, t)
+    some = torch.cat((torch.arange(20), torch.arange(tokens // 2 - 10, tokens // 2 + 10), torch.arange(tokens - 20, tokens)))
+    at = some.cuda()
+    ref = R.xent(x[at].cpu(), w.cpu(), t[at].cpu(), -100)
+    _close(lse[at], ref["lse"], ref["e_loss"], "lse")
+    _close(loss[at], ref["loss"], ref["e_loss"], "loss")
+    assert bool(torch.isfinite(loss).all())
 
 
 def test_two_streams_at_once():
