@@ -54,7 +54,7 @@ int check_xent(const DionXentDesc* d, int op) {
   if (d->ld_hidden < d->hidden || d->ld_weight < d->hidden)
     return fail(DION_E_INVALID, "ld_hidden = %lld, ld_weight = %lld", static_cast<long long>(d->ld_hidden),
                 static_cast<long long>(d->ld_weight));
-  if (d->vocab_start < 0 || d->vocab_start + d->vocab > d->vocab_total)
+  if (d->vocab_start < 0 || d->vocab_total < d->vocab || d->vocab_start > d->vocab_total - d->vocab)
     return fail(DION_E_INVALID, "words %lld .. + %d of %lld", static_cast<long long>(d->vocab_start), d->vocab,
                 static_cast<long long>(d->vocab_total));
   return DION_OK;

@@ -62,6 +62,13 @@ def _rows(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
     return rows, cols, ld or cols
 
 
+def _fits(bits: int, **sizes: int) -> None:
+    """What goes into a descriptor's field of `bits` bits, which would keep the low ones of a larger number."""
+    for what, n in sizes.items():
+        if not -(1 << (bits - 1)) <= n < 1 << (bits - 1):
+            raise RuntimeError(f"[DION_BAD_SIZE] {what}={n} does not fit {bits} bits")
+
+
 def _like(t: torch.Tensor, what: str, like: torch.Tensor) -> int:
     """The row stride of `t`, which has to be a tensor like `like`."""
     if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
@@ -164,6 +171,7 @@ class RmsNormAddGrads(NamedTuple):
 @functools.lru_cache(maxsize=512)
 def _norm_desc(rows, cols, dtype, w_dtype, gw_dtype, y_dtype, scale_block, accumulate, eps, p, *lds):
     """The descriptor of a call (read only: calls of the same shapes share it) and its scratch."""
+    _fits(32, cols=cols)
     d = _lm_lib.DionNormDesc(rows, cols, dtype, w_dtype, gw_dtype, y_dtype, scale_block, accumulate, eps, p, *lds)
     nbytes = ctypes.c_size_t(0)
     _lm_lib.check(_lm_lib.load().dion_rms_norm_add_workspace_bytes(_byref(d), _byref(nbytes)),
@@ -183,7 +191,7 @@ def rms_norm_add_forward(x: torch.Tensor, weight: torch.Tensor, residual: Option
                          scale_block: int = 0) -> RmsNormAdd:
     """`h = residual + dropout(x)`, rounded to x's dtype; `y = h * rsqrt(mean(h^2) + eps) * weight`.
 
-    `scale_block` > 0 (at least 8, or all columns; -1: one block a row): y is float8_e4m3fn, each block
+    Rows of up to 16384 columns.  `scale_block` > 0 (at least 8, or all columns; -1: one block a row): y is float8_e4m3fn, each block
     of that many columns over its own fp32 `scale` = max |y| / 448 (at least 2^-126), so that
     `y.float() * scale` restores it.  Dropout as in `dropout_add_forward`."""
     rows, cols, ld = _rows(x, "x")
@@ -271,6 +279,8 @@ def rms_norm_add_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.T
 def _xent_shape(op, tokens, hidden, vocab, dtype, gw_dtype, accumulate, pack_weight, start, total, ignore, ld_hidden,
                 ld_weight, ld_grad_weight, piece_bytes):
     """The descriptor of a call (read only: calls of the same shapes share it) and its scratch."""
+    _fits(32, hidden=hidden, vocab=vocab)
+    _fits(64, vocab_start=start, vocab_size=total, ignore_index=ignore, piece_bytes=piece_bytes)
     d = _lm_lib.DionXentDesc(tokens, hidden, vocab, dtype, gw_dtype, accumulate, pack_weight, start, total, ignore,
                              ld_hidden, ld_weight, hidden, ld_grad_weight, piece_bytes)
     nbytes = ctypes.c_size_t(0)
@@ -320,7 +330,8 @@ def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, tar
     """(loss, lse), fp32 of target's shape: the cross entropy of `hidden @ weight.T` at each token and
     the logarithm of its softmax's denominator (for the backward pass).  The logits are never stored.
 
-    hidden (..., H) and weight (V, H) are bf16 or fp32 alike, target int64.  A token whose target is
+    hidden (..., H) and weight (V, H) are bf16 or fp32 alike, target int64; up to 2^24 tokens, H 2^20, V
+    2^21.  An infinity in fp32 inputs makes the logits it meets NaN (they are split into limbs).  A token whose target is
     `ignore_index` costs nothing: its loss and lse are 0 and its hidden state is not read.  Any other
     target outside the vocabulary gives a NaN loss.
 
@@ -355,11 +366,12 @@ def linear_cross_entropy_backward(grad_loss: torch.Tensor, hidden: torch.Tensor,
                                   ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(grad_hidden, grad_weight) for the upstream gradient `grad_loss` (fp32, target's shape).
 
-    The logits are made again a piece of the vocabulary at a time; at most `piece_bytes` (0:
-    1 GiB) of their gradient is held.  Tokens that are ignored or whose grad_loss is 0 take no part.  `grad_weight` (fp32 or bf16,
-    e.g. `weight.main_grad`) is written, or with `accumulate` added to, rows past `vocab_size` as zeros;
-    without it a new tensor of weight's dtype is returned.  The logits' gradient is rounded to bf16 for
-    the matrix cores where the result is bf16, and to two fp16 limbs (2^-22) where it is fp32.  With `group`, grad_hidden is summed over the vocabulary's shards."""
+    The logits are made again a piece of the vocabulary at a time; at most `piece_bytes` (0: 1 GiB) of
+    their gradient is held.  Tokens that are ignored or whose grad_loss is 0 take no part.
+    `grad_weight` (fp32 or bf16, e.g. `weight.main_grad`) is written, or with `accumulate` added to, rows
+    past `vocab_size` as zeros; without it a new tensor of weight's dtype is returned.  The logits'
+    gradient is rounded to bf16 for the matrix cores where the result is bf16, and to two fp16 limbs
+    (2^-22) where it is fp32.  With `group`, grad_hidden is summed over the vocabulary's shards."""
     gw = _grad_weight(weight, grad_weight, accumulate, "grad_weight") if need_weight else None
     d, nbytes = _xent_desc(_lm_lib.XENT_BACKWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index, gw,
                            accumulate, piece_bytes)

@@ -82,7 +82,8 @@ def _xent_desc(**kw):
     ({"vocab_start": 1}, _lib.DION_E_INVALID), ({"ld_weight": 63}, _lib.DION_E_INVALID),
     ({"ld_hidden": 63}, _lib.DION_E_INVALID), ({"dtype": 3}, _lib.DION_E_UNSUPPORTED),
     ({"gw_dtype": 0}, _lib.DION_E_UNSUPPORTED), ({"ld_weight": 1 << 22}, _lib.DION_E_UNSUPPORTED),
-    ({"tokens": 1 << 25}, _lib.DION_E_UNSUPPORTED), ({"piece_bytes": -1}, _lib.DION_E_INVALID)])
+    ({"tokens": 1 << 25}, _lib.DION_E_UNSUPPORTED),
+    ({"vocab_start": (1 << 63) - 1}, _lib.DION_E_INVALID), ({"vocab_total": -(1 << 63)}, _lib.DION_E_INVALID), ({"piece_bytes": -1}, _lib.DION_E_INVALID)])
 def test_xent_workspace_query_refuses(kw, code):
     n = ctypes.c_size_t(0)
     assert _lm_lib.load().dion_xent_workspace_bytes(ctypes.byref(_xent_desc(**kw)), _lm_lib.XENT_BACKWARD,
@@ -171,6 +172,20 @@ def test_python_calls_refuse():
         lm_ops._grad_weight(w, None, True, "grad_weight")
     with pytest.raises(RuntimeError, match="DION_BAD_GRAD_OUT"):
         lm_ops._grad_weight(w, torch.zeros(4, 8), False, "grad_weight")
+
+
+def test_sizes_that_a_descriptor_cannot_hold():
+    """ctypes would keep the low bits: 2^32 + 8 columns would be taken for 8."""
+    big = (1 << 32) + 8
+    with pytest.raises(RuntimeError, match="DION_BAD_SIZE.*cols"):
+        lm_ops._norm_desc(1, big, 2, 1, 1, 2, 0, 0, 1e-5, 0.0, big, 0, big, big)
+    base = dict(op=1, tokens=1, hidden=8, vocab=8, dtype=2, gw_dtype=2, accumulate=0, pack_weight=0, start=0, total=8,
+                ignore=-100, ld_hidden=8, ld_weight=8, ld_grad_weight=8, piece_bytes=0)
+    assert lm_ops._xent_shape(*base.values())[1] > 0
+    for k, v in (("hidden", big), ("vocab", big), ("start", 1 << 63), ("total", 1 << 64), ("ignore", 1 << 63),
+                 ("piece_bytes", 1 << 64)):
+        with pytest.raises(RuntimeError, match="DION_BAD_SIZE"):
+            lm_ops._xent_shape(*{**base, k: v}.values())
 
 
 def _shards(rank, world, port, ret):
