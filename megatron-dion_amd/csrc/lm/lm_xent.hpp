@@ -16,12 +16,12 @@
 //
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
 // whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, one
-// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is fp32: grad_weight into
-// an fp32 main_grad (4096 tokens x 768 x 50257: 1.87 ms a pass, 2.34 with three bf16 limbs; two bf16 limbs
-// left 2.6e-6 of the 2-norm, twice what an fp32 product is off), and everything for fp32 inputs, which are two fp16
-// limbs themselves.  The power of two that brings such an operand into fp16's range comes from its
-// largest finite value; g's is known, |p - [v = y]| <= 1 times the mantissa of the token's gl, whose
-// power of two goes into X (for dW) or is put back at the end (for dX).
+// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is
+// fp32: grad_weight into an fp32 main_grad (4096 tokens x 768 x 50257: 1.87 ms a pass, 2.34 with three
+// bf16 limbs; two bf16 limbs left 2.6e-6 of the 2-norm, twice what an fp32 product is off), and everything
+// for fp32 inputs, which are two fp16 limbs themselves.  The power of two that brings such an operand
+// into fp16's range comes from its largest finite value; g's is known, |p - [v = y]| <= 1 times the
+// mantissa of the token's gl, whose power of two goes into X (for dW) or is put back at the end (for dX).
 
 namespace xent {
 
@@ -786,7 +786,8 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       a.out_vec = d->hidden % 4 == 0 && d->ld_grad_weight % 4 == 0 && aligned16(grad_weight);
       // tiles stay inside the piece of g (a multiple of 256 words): what lies past n there makes rows
       // that are not stored
-      rc = launch<true, true, EPI_OUT>(p.dw_limbs > 0, pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2), a, n, d->hidden, st, "xent(grad weight)");
+      const int tile = pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2);
+      rc = launch<true, true, EPI_OUT>(p.dw_limbs > 0, tile, a, n, d->hidden, st, "xent(grad weight)");
       if (rc != DION_OK) return rc;
     }
   }

@@ -191,9 +191,9 @@ def rms_norm_add_forward(x: torch.Tensor, weight: torch.Tensor, residual: Option
                          scale_block: int = 0) -> RmsNormAdd:
     """`h = residual + dropout(x)`, rounded to x's dtype; `y = h * rsqrt(mean(h^2) + eps) * weight`.
 
-    Rows of up to 16384 columns.  `scale_block` > 0 (at least 8, or all columns; -1: one block a row): y is float8_e4m3fn, each block
-    of that many columns over its own fp32 `scale` = max |y| / 448 (at least 2^-126), so that
-    `y.float() * scale` restores it.  Dropout as in `dropout_add_forward`."""
+    Rows of up to 16384 columns.  `scale_block` > 0 (at least 8, or all columns; -1: one block a row): y
+    is float8_e4m3fn, each block of that many columns over its own fp32 `scale` = max |y| / 448 (at least
+    2^-126), so that `y.float() * scale` restores it.  Dropout as in `dropout_add_forward`."""
     rows, cols, ld = _rows(x, "x")
     ld_r = 0 if residual is None else _like(residual, "residual", x)
     device = x.device
