@@ -260,15 +260,23 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a, const float
     pack8<T>(a, i, rows, a.index, mul);
 }
 
-// select and the packs in one launch, for few tokens: every block numbers the tokens for itself (a round
-// or two of 1024), the first one writes it down.  x: hidden states for z, xg: for dW (fp16), w: the
+// select and the packs in one launch, for few tokens: each of the first `tok_blocks` blocks numbers the
+// tokens for itself (a round of 4096) and gathers a share of their rows, and the first one writes the
+// numbers down; the others pack the weight.  x: hidden states for z, xg: for dW (fp16), w: the
 // weight's first piece (0 rows: none).
 constexpr int kFewTokens = 2048;
 
 template <typename T>
 __global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const PackArgs x, const PackArgs xg,
-                                                       const PackArgs w, int amax_blocks) {
+                                                       const PackArgs w, int amax_blocks, int tok_blocks) {
   __shared__ int index[kFewTokens];
+  if (static_cast<int>(blockIdx.x) >= tok_blocks) {
+    const float mul = w.f16 ? scale_of(block_amax(a.out.amax + kAmaxBlocks, amax_blocks)) : 1.0f;
+    const int64_t n = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8), step = static_cast<int64_t>(gridDim.x - tok_blocks) * 1024;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - tok_blocks) * 1024 + threadIdx.x; i < n; i += step)
+      pack8<T>(w, i, w.rows, nullptr, mul);
+    return;
+  }
   const int count = select(a, [&](int t, int n) {
     if (n >= 0) index[n] = t;
     if (blockIdx.x == 0) put_token(a, t, n);
@@ -284,13 +292,11 @@ __global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const
   }
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.out.count = count;
-  const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), ng = static_cast<int64_t>(xg.rows_p) * (xg.cols_p / 8),
-                nw = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + ng + nw;
-       i += static_cast<int64_t>(gridDim.x) * 1024) {
+  const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), ng = static_cast<int64_t>(xg.rows_p) * (xg.cols_p / 8);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + ng;
+       i += static_cast<int64_t>(tok_blocks) * 1024) {
     if (i < nx) pack8<T>(x, i, count, index, mul[0]);
-    else if (i < nx + ng) pack8<T>(xg, i - nx, count, index, mul[2]);
-    else pack8<T>(w, i - nx - ng, w.rows, nullptr, mul[1]);
+    else pack8<T>(xg, i - nx, count, index, mul[2]);
   }
 }
 
@@ -347,7 +353,8 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
     const int p = tok.pos[t];
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (p >= 0) {
-      for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {  // four in flight
         float q[8];
         load_vec<8>(slab + s * stride + static_cast<int64_t>(p) * ldslab + c, q);
 #pragma unroll
@@ -636,11 +643,12 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   }
   if (p.pack_w) w = weight_args(d, p, weight, 0, d->vocab < p.piece ? d->vocab : p.piece, ws);
   if (d->tokens <= kFewTokens) {
-    const long units = static_cast<long>(x.rows_p + xg.rows_p) * (x.cols_p / 8) + static_cast<long>(w.rows_p) * (w.cols_p / 8);
-    const long blocks = ceil_div(units, 1024);
-    const dim3 grid(blocks < 512 ? blocks : 512);  // as many as run at once: each numbers the tokens first
-    if (p.f32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks);
-    else hipLaunchKernelGGL(prepare_kernel<bf16>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks);
+    const long xb = ceil_div(static_cast<long>(x.rows_p + xg.rows_p) * (x.cols_p / 8), 1024);
+    const long wb = ceil_div(static_cast<long>(w.rows_p) * (w.cols_p / 8), 1024);
+    const int tb = static_cast<int>(xb < 512 ? xb : 512);  // as many as run at once: each numbers the tokens first
+    const dim3 grid(tb + (wb < 2048 ? wb : 2048));
+    if (p.f32) hipLaunchKernelGGL(prepare_kernel<float>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks, tb);
+    else hipLaunchKernelGGL(prepare_kernel<bf16>, grid, dim3(1024), 0, st, a, x, xg, w, p.amax_blocks, tb);
     return check_launch("xent(prepare)");
   }
   hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a, p.amax_blocks);
