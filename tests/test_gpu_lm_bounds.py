@@ -1,0 +1,48 @@
+"""The training operators on the GPU at the ends of their ranges: what each rounding may cost, and no more."""
+import pytest
+import torch
+
+import megatron_dion_amd as mda
+from tests import _lm_reference as R
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+# ------------------------------------------------------------------------------- norm in 8 bits
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("cols,block", [(128, 128), (4096, 128), (4096, -1), (4096, 96), (1000, 128), (999, 100), (16, 8)])
+def test_norm_in_8_bits_is_the_quotient_rounded(dtype, cols, block):
+    """y / s, rounded to fp32 and then to e4m3, code for code.  A row of +-1 with eps = 0 has rstd = 1, so y is +-w
+    exactly; the weights are the middles of two codes times a scale that is no power of two, where a rounding more
+    changes the code."""
+    g = torch.Generator().manual_seed(cols)
+    codes = torch.arange(0, 0x7F, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    middles = (codes[1:] + codes[:-1]) / 2
+    b = cols if block < 0 else block
+    n = -(-cols // b)
+    for size in [1.0] * 8 + [2.0 ** -80, 2.0 ** -95, 2.0 ** -115, 2.0 ** 100]:
+        top = 448.0 * size * (1.0 + torch.rand(n, generator=g))
+        s = (top / 448.0).clamp_min(2.0 ** -126)  # fp32, as the operator takes it from the block's largest
+        w = middles[torch.randint(0, len(middles), (n, b), generator=g)] * s[:, None]
+        w[:, 0] = top
+        w = w.view(-1)[:cols].contiguous()
+        x = torch.where(torch.rand(3, cols, generator=g) < 0.5, -1.0, 1.0).to(dtype)
+        f = mda.rms_norm_add_forward(x.cuda(), w.cuda(), eps=0.0, scale_block=block)
+        assert (f.rstd == 1.0).all()
+        assert torch.equal(f.scale.cpu(), s.expand(3, n))
+        want = (w / s.repeat_interleave(b)[:cols]).clamp(-448.0, 448.0) * x.float()
+        want = want.to(torch.float8_e4m3fn)
+        assert torch.equal(f.y.cpu().view(torch.uint8), want.view(torch.uint8)), size
+
+
+def test_norm_in_8_bits_of_a_block_with_an_infinity():
+    """The scale is infinite: the infinity itself becomes NaN, the rest of its block 0."""
+    x = torch.ones(1, 256)
+    w = torch.ones(256)
+    w[3] = float("inf")
+    for block in (128, 96):
+        f = mda.rms_norm_add_forward(x.cuda(), w.cuda(), eps=0.0, scale_block=block)
+        y = f.y.float().cpu()[0]
+        assert torch.isnan(y).nonzero()[:, 0].tolist() == [3]
+        assert (y[:3] == 0).all() and (y[4:block] == 0).all() and (y[block:] == 448).all()
