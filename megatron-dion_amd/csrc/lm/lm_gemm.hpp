@@ -223,15 +223,17 @@ __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// 2^e <= |x| < 2^(e + 1) as 2^e (1 for 0, infinities and NaN)
-__device__ __forceinline__ float pow2_below(float x) {
+// e with 2^e <= |x| < 2^(e + 1) (0 for 0, infinities and NaN), and 2^e
+__device__ __forceinline__ int exp_below(float x) {
   const float v = fabsf(x);
-  if (!(v > 0.0f && v <= 3.402823466e38f)) return 1.0f;
+  if (!(v > 0.0f && v <= 3.402823466e38f)) return 0;
   int e;
   frexpf(v, &e);
-  return ldexpf(1.0f, e - 1);
+  return e - 1;
 }
-constexpr float kGradScale = 8192.0f;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
+__device__ __forceinline__ float pow2_below(float x) { return ldexpf(1.0f, exp_below(x)); }
+constexpr int kGradExp = 13;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
+constexpr float kGradScale = 1 << kGradExp;
 
 // The loop over steps of 64 k is software-pipelined by hand.  A step is four phases of 16 k; in each,
 // a wave's MFMAs run on fragments in registers while it reads the next phase's from LDS.  The barrier
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
       if (live) {
         tgt = a.tgt[row] - a.col0 - cw;
         gl = a.gl[row];
-        gm = gl * (kGradScale / pow2_below(gl));
+        gm = ldexpf(gl, kGradExp - exp_below(gl));  // exponents add: 2^13 / 2^e is past fp32 for gl below 2^-114
         const float lse = a.lse[row];
         l2 = lse * kLog2e;  // and what it lacks, so that p is not off by the rounding of a large lse
         l2lo = fmaf(lse, kLog2e, -l2);

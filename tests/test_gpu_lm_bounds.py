@@ -46,3 +46,51 @@ def test_norm_in_8_bits_of_a_block_with_an_infinity():
         y = f.y.float().cpu()[0]
         assert torch.isnan(y).nonzero()[:, 0].tolist() == [3]
         assert (y[:3] == 0).all() and (y[4:block] == 0).all() and (y[block:] == 448).all()
+
+
+# ------------------------------------------------------------------------------- linear cross entropy
+def _randn(seed, *shape, scale=1.0, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def _close(got, want, tol, what):
+    got, want = got.detach().double().cpu(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst " \
+                          f"{float(((got - want).abs() / (tol + 1e-300)).nan_to_num(1e30).max()):.3g} times the bound"
+
+
+def _case(tokens, hidden, vocab, dtype, seed=0):
+    x = _randn(seed, tokens, hidden, dtype=dtype)
+    w = _randn(seed + 1, vocab, hidden, scale=2 * hidden ** -0.5, dtype=dtype)
+    g = torch.Generator().manual_seed(seed + 2)
+    t = torch.randint(0, vocab, (tokens,), generator=g)
+    return x, w, t, torch.rand(tokens, generator=g) / tokens
+
+
+def _check(x, w, t, gl, out_dtype):
+    ref = R.xent(x, w, t, -100, gl, out_dtype=out_dtype)
+    xc, wc, tc = x.cuda(), w.cuda(), t.cuda()
+    loss, lse = mda.linear_cross_entropy_forward(xc, wc, tc)
+    _close(loss, ref["loss"], ref["e_loss"], "loss")
+    gw = torch.full(w.shape, float("nan"), dtype=out_dtype, device="cuda")
+    dx, dw = mda.linear_cross_entropy_backward(gl.cuda(), xc, wc, tc, lse, grad_weight=gw)
+    # half the spacing of bf16's least numbers, for each g and for the result; fp32's is in the reference's bounds
+    low = 2.0 ** -134 if x.dtype == BF16 else 0.0
+    _close(dx, ref["grad_hidden"], ref["e_grad_hidden"] + low * (1 + w.double().abs().sum(0)), "grad_hidden")
+    low_out = 2.0 ** -134 if out_dtype == BF16 else 0.0
+    _close(dw, ref["grad_weight"], ref["e_grad_weight"] + low * x.double().abs().sum(0) + low_out, "grad_weight")
+
+
+TYPES = [(BF16, BF16), (BF16, F32), (F32, F32)]
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+@pytest.mark.parametrize("tokens", [8, 200, 600])
+def test_xent_of_tiny_upstream_gradients(dtype, out_dtype, tokens):
+    """Tokens whose upstream gradient is tiny or subnormal, among ordinary ones."""
+    x, w, t, gl = _case(tokens, 64, 300, dtype)
+    gl[1], gl[2], gl[4], gl[5] = 1e-34, -1e-36, 1e-42, 1.5e-45
+    _check(x, w, t, gl, out_dtype)
