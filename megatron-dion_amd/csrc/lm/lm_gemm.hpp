@@ -53,7 +53,7 @@ struct GemmArgs {
   const int* tgt;        // per compact token: column of its target within the shard, -1: none
   const float* lse;      // per compact token
   const float* gl;       // per compact token: upstream gradient
-  const float* scale;    // device: what undoes the operands' scales, NULL: 1
+  const int* scale;      // device: the exponent of the power of two that undoes the operands' scales, NULL: 0
   int col0;              // first shard column of this piece
   float2* part;          // stats: [part][token] (c, sum of 2^(x log2(e) - c))
   float* tlogit;         // stats: per compact token
@@ -223,7 +223,7 @@ __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// e with 2^e <= |x| < 2^(e + 1) (0 for 0, infinities and NaN), and 2^e
+// e with 2^e <= |x| < 2^(e + 1) (0 for 0, infinities and NaN)
 __device__ __forceinline__ int exp_below(float x) {
   const float v = fabsf(x);
   if (!(v > 0.0f && v <= 3.402823466e38f)) return 0;
@@ -231,9 +231,7 @@ __device__ __forceinline__ int exp_below(float x) {
   frexpf(v, &e);
   return e - 1;
 }
-__device__ __forceinline__ float pow2_below(float x) { return ldexpf(1.0f, exp_below(x)); }
 constexpr int kGradExp = 13;  // |p - [v = y]| < 1 and the mantissa of gl below 2: under 2^14
-constexpr float kGradScale = 1 << kGradExp;
 
 // The loop over steps of 64 k is software-pipelined by hand.  A step is four phases of 16 k; in each,
 // a wave's MFMAs run on fragments in registers while it reads the next phase's from LDS.  The barrier
@@ -362,7 +360,9 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
   const int hi = lane >> 5, hi4 = hi * 4;
   const int cw = c0 + wc * WC;
   const bool whole = c0 + BC <= a.cols;  // no column of the tile is past the end
-  const float scale = a.scale ? *a.scale : 1.0f;
+  const int scale_exp = a.scale ? *a.scale : 0;
+  // of logits, where an exponent past fp32's would make a NaN of 0: what such a logit is does not matter
+  const float scale = ldexpf(1.0f, scale_exp < -126 ? -126 : scale_exp > 126 ? 126 : scale_exp);
   const float l2e = kLog2e * scale;      // exact: scale is a power of two
   if constexpr (EPI == EPI_STATS) {
     // Exponentials to base 2: x log2(e) - c is one fma, and c (the rounded maximum) one exact number in
@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
           *o = v;
         }
       } else if (orow < a.rows && col < a.cols) {
-        v *= scale;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], scale_exp);
         const int64_t at = static_cast<int64_t>(orow) * a.ldo + col;
         if (a.out_bf16) {
           uint16_t* o = static_cast<uint16_t*>(a.out) + at;

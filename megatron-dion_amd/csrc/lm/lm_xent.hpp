@@ -34,11 +34,11 @@ struct Tokens {  // compact arrays, by the number a token has among those that t
   float* gl;     // [tokens_p] (backward)
   float* tlogit; // [tokens_p] (forward)
   float* delta;  // [tokens_p] (backward, bf16 inputs): what the target's g lost when it was rounded
-  float* amax;   // [3][kAmaxBlocks]: largest |X|, |W|, |X| 2^e of a block's share
-  float* scale;  // [4]: kScaleZ ...
+  float* amax;   // [3][kAmaxBlocks]: largest |X|, |W| of a block's share, and of |X| 2^e the exponent + kExpBias
+  int* scale;    // [4]: kScaleZ ...
 };
 constexpr int kAmaxBlocks = 512;
-// what undoes the scales of z = X W^T, dX = g W (without the token's 2^e), dW = g^T X
+// exponents of what undoes the scales of z = X W^T, dX = g W (without the token's 2^e), dW = g^T X
 enum { kScaleZ = 0, kScaleDx = 1, kScaleDw = 2 };
 
 struct SelectArgs {
@@ -115,18 +115,17 @@ struct PackArgs {
   int rows_p, cols_p;  // packed extents, zeros outside the source
   uint16_t* dst;       // limbs one after the other
   int nlimb;
-  int f16;             // fp16 limbs of the values times `mul` (a parameter), else one bf16
+  int f16;             // fp16 limbs of the values times a power of two, else one bf16
   int amax;            // f16: which row of Tokens::amax
   const float* gl;     // not NULL: times the power of two below |gl| of the row's token, too
 };
 
-// 2^s that brings m under 2^15
-__device__ __forceinline__ float scale_of(float m) {
-  if (!(m > 0.0f)) return 1.0f;
-  int e;
-  frexpf(m, &e);  // m < 2^e
-  e = 15 - e;
-  return ldexpf(1.0f, e < -100 ? -100 : e > 100 ? 100 : e);
+// Scales are held as exponents and applied by ldexp: with fp32's whole range in the inputs, 2^s, 2^-s and
+// 2^(s + e) are past it.  s that brings m under 2^15, from m and from its exponent.
+constexpr int kExpBias = 1024;
+__device__ __forceinline__ int scale_of(float m) { return m > 0.0f ? 14 - exp_below(m) : 0; }
+__device__ __forceinline__ int scale_of_exp(float biased) {
+  return biased > 0.0f ? 14 - (static_cast<int>(biased) - kExpBias) : 0;
 }
 
 // the largest of a row of Tokens::amax; the whole block takes part
@@ -167,7 +166,7 @@ __device__ __forceinline__ float amax8(const T* p, int c, int cols) {
   return m;
 }
 
-// Each block's share of the largest |X| (tokens that take part), |X| 2^e and |W|.
+// Each block's share of the largest |X| (tokens that take part), |W|, and the exponent of |X| 2^e.
 template <typename T>
 __global__ void __launch_bounds__(256) amax_kernel(const AmaxArgs a) {
   __shared__ float red[4];
@@ -180,14 +179,14 @@ __global__ void __launch_bounds__(256) amax_kernel(const AmaxArgs a) {
       if (a.target[t] == a.ignore || (a.gl && a.gl[t] == 0.0f)) continue;
       const float m = amax8(static_cast<const T*>(a.x) + t * a.ldx, c, a.hidden);
       mx = fmaxf(mx, m);
-      if (a.want_xg) mg = fmaxf(mg, m * pow2_below(a.gl[t]));
+      if (a.want_xg && m > 0.0f) mg = fmaxf(mg, static_cast<float>(exp_below(m) + exp_below(a.gl[t]) + kExpBias));
     }
   if (a.want_w)
     for (int64_t i = first; i < static_cast<int64_t>(a.vocab) * per; i += step) {
       const int t = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(t) * per) * 8;
       mw = fmaxf(mw, amax8(static_cast<const T*>(a.w) + t * a.ldw, c, a.hidden));
     }
-  float v[3] = {mx, mw, mg <= 3.402823466e38f ? mg : 3.402823466e38f};
+  float v[3] = {mx, mw, mg};
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
 #pragma unroll
@@ -199,9 +198,9 @@ __global__ void __launch_bounds__(256) amax_kernel(const AmaxArgs a) {
   }
 }
 
-// 8 columns of a row of src, `i`: which; f16: times mul
+// 8 columns of a row of src, `i`: which; f16: times 2^s
 template <typename T>
-__device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, const int* index, float mul) {
+__device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, const int* index, int s2) {
   const int per = a.cols_p / 8;
   const int row = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<int64_t>(row) * per) * 8;
   float v[8];
@@ -214,9 +213,9 @@ __device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, co
   uint16_t* o = a.dst + static_cast<int64_t>(row) * a.cols_p + c;
   u32x4 q;
   if (a.f16) {
-    const float e2 = a.gl && row < rows ? pow2_below(a.gl[index[row]]) : 1.0f;
+    if (a.gl && row < rows) s2 += exp_below(a.gl[index[row]]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] * e2 * mul;  // in this order as the maximum was taken: no overflow
+    for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], s2);
     for (int l = 0; l < a.nlimb; ++l) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -234,11 +233,11 @@ __device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, co
   }
 }
 
-// What undoes the scales (one thread).
-__device__ __forceinline__ void put_scales(float* scale, float mx, float mw, float mg) {
-  scale[kScaleZ] = (1.0f / scale_of(mx)) * (1.0f / scale_of(mw));
-  scale[kScaleDx] = (1.0f / kGradScale) * (1.0f / scale_of(mw));
-  scale[kScaleDw] = (1.0f / kGradScale) * (1.0f / scale_of(mg));
+// What undoes the scales 2^sx, 2^sw, 2^sg (one thread).
+__device__ __forceinline__ void put_scales(int* scale, int sx, int sw, int sg) {
+  scale[kScaleZ] = -sx - sw;
+  scale[kScaleDx] = -kGradExp - sw;
+  scale[kScaleDw] = -kGradExp - sg;
 }
 
 __global__ void __launch_bounds__(1024) select_kernel(const SelectArgs a, int amax_blocks) {
@@ -247,17 +246,21 @@ __global__ void __launch_bounds__(1024) select_kernel(const SelectArgs a, int am
   if (amax_blocks) {
     const float mx = block_amax(a.out.amax, amax_blocks), mw = block_amax(a.out.amax + kAmaxBlocks, amax_blocks),
                 mg = block_amax(a.out.amax + 2 * kAmaxBlocks, amax_blocks);
-    if (threadIdx.x == 0) put_scales(a.out.scale, mx, mw, mg);
+    if (threadIdx.x == 0) put_scales(a.out.scale, scale_of(mx), scale_of(mw), scale_of_exp(mg));
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a, const float* amax, int amax_blocks) {
   const int rows = a.index ? *a.count : a.rows;
-  const float mul = a.f16 ? scale_of(block_amax(amax + a.amax * kAmaxBlocks, amax_blocks)) : 1.0f;
+  int s2 = 0;
+  if (a.f16) {
+    const float m = block_amax(amax + a.amax * kAmaxBlocks, amax_blocks);
+    s2 = a.amax == 2 ? scale_of_exp(m) : scale_of(m);
+  }
   const int64_t n = static_cast<int64_t>(a.rows_p) * (a.cols_p / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-    pack8<T>(a, i, rows, a.index, mul);
+    pack8<T>(a, i, rows, a.index, s2);
 }
 
 // select and the packs in one launch, for few tokens: each of the first `tok_blocks` blocks numbers the
@@ -272,32 +275,33 @@ __global__ void __launch_bounds__(1024) prepare_kernel(const SelectArgs a, const
                                                        const PackArgs w, int amax_blocks, int tok_blocks) {
   __shared__ int index[kFewTokens];
   if (static_cast<int>(blockIdx.x) >= tok_blocks) {
-    const float mul = w.f16 ? scale_of(block_amax(a.out.amax + kAmaxBlocks, amax_blocks)) : 1.0f;
+    const int s2 = w.f16 ? scale_of(block_amax(a.out.amax + kAmaxBlocks, amax_blocks)) : 0;
     const int64_t n = static_cast<int64_t>(w.rows_p) * (w.cols_p / 8), step = static_cast<int64_t>(gridDim.x - tok_blocks) * 1024;
     for (int64_t i = static_cast<int64_t>(blockIdx.x - tok_blocks) * 1024 + threadIdx.x; i < n; i += step)
-      pack8<T>(w, i, w.rows, nullptr, mul);
+      pack8<T>(w, i, w.rows, nullptr, s2);
     return;
   }
   const int count = select(a, [&](int t, int n) {
     if (n >= 0) index[n] = t;
     if (blockIdx.x == 0) put_token(a, t, n);
   });
-  float mul[3] = {1.0f, 1.0f, 1.0f};
+  int s2[3] = {0, 0, 0};
   if (amax_blocks) {
 #pragma unroll
     for (int k = 0; k < 3; ++k)
-      if (k == 2 ? xg.rows_p > 0 : x.f16 != 0) mul[k] = block_amax(a.out.amax + k * kAmaxBlocks, amax_blocks);
-    if (blockIdx.x == 0 && threadIdx.x == 0) put_scales(a.out.scale, mul[0], mul[1], mul[2]);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) mul[k] = scale_of(mul[k]);
+      if (k == 2 ? xg.rows_p > 0 : x.f16 != 0) {
+        const float m = block_amax(a.out.amax + k * kAmaxBlocks, amax_blocks);
+        s2[k] = k == 2 ? scale_of_exp(m) : scale_of(m);
+      }
+    if (blockIdx.x == 0 && threadIdx.x == 0) put_scales(a.out.scale, s2[0], s2[1], s2[2]);
   }
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.out.count = count;
   const int64_t nx = static_cast<int64_t>(x.rows_p) * (x.cols_p / 8), ng = static_cast<int64_t>(xg.rows_p) * (xg.cols_p / 8);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x; i < nx + ng;
        i += static_cast<int64_t>(tok_blocks) * 1024) {
-    if (i < nx) pack8<T>(x, i, count, index, mul[0]);
-    else pack8<T>(xg, i - nx, count, index, mul[2]);
+    if (i < nx) pack8<T>(x, i, count, index, s2[0]);
+    else pack8<T>(xg, i - nx, count, index, s2[2]);
   }
 }
 
@@ -345,7 +349,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float2* part, int parts
 // put back in fp32, from one row of W.
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(const float* slab, int splits, int64_t stride, int64_t ldslab,
-                                                    int tokens, int cols, const float* scale, const Tokens tok,
+                                                    int tokens, int cols, const int* scale, const Tokens tok,
                                                     const T* w, int64_t ldw, T* out, int64_t ldo) {
   const int per = (cols + 7) / 8;
   const int64_t n = static_cast<int64_t>(tokens) * per;
@@ -361,10 +365,10 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += q[k];
       }
-      if (scale) {  // one after the other: their product may underflow
-        const float u = *scale, e2 = pow2_below(tok.gl[p]);
+      if (scale) {
+        const int e2 = *scale + exp_below(tok.gl[p]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = v[k] * u * e2;
+        for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], e2);
       }
       const float lost = w ? tok.delta[p] : 0.0f;
       if (lost != 0.0f) {
@@ -546,7 +550,7 @@ Tokens tokens_at(char* ws, const Plan& p) {
   char* b = ws + p.tok;
   const size_t n = static_cast<size_t>(p.tokens_p);
   t.count = reinterpret_cast<int*>(b);
-  t.scale = reinterpret_cast<float*>(b + 256);
+  t.scale = reinterpret_cast<int*>(b + 256);
   t.amax = reinterpret_cast<float*>(b + 512);
   t.pos = reinterpret_cast<int*>(t.amax + 3 * kAmaxBlocks);
   t.index = t.pos + n;
@@ -812,7 +816,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     else
       hipLaunchKernelGGL(round_kernel<bf16>, grid, dim3(256), 0, st, slab, p.splits, sstride,
                          static_cast<int64_t>(p.hidden_p), static_cast<int>(d->tokens), d->hidden,
-                         static_cast<const float*>(nullptr), tok, static_cast<const bf16*>(weight), d->ld_weight,
+                         static_cast<const int*>(nullptr), tok, static_cast<const bf16*>(weight), d->ld_weight,
                          static_cast<bf16*>(grad_hidden), d->ld_grad_hidden);
     rc = check_launch("xent(round grad hidden)");
   }

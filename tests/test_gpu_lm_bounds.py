@@ -94,3 +94,34 @@ def test_xent_of_tiny_upstream_gradients(dtype, out_dtype, tokens):
     x, w, t, gl = _case(tokens, 64, 300, dtype)
     gl[1], gl[2], gl[4], gl[5] = 1e-34, -1e-36, 1e-42, 1.5e-45
     _check(x, w, t, gl, out_dtype)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", TYPES)
+def test_xent_of_tiny_upstream_gradients_alone(dtype, out_dtype):
+    """All of them far below 1: their powers of two leave the hidden states' limbs all their bits."""
+    for scale in (1e-30, 1e-35):
+        x, w, t, gl = _case(100, 64, 300, dtype)
+        _check(x, w, t, gl * scale, out_dtype)
+
+
+@pytest.mark.parametrize("tokens", [40, 2500])
+@pytest.mark.parametrize("scale", [1e37, 1e36, 1e33, 1e-33, 1e-36, 1e-37])
+def test_xent_fp32_to_the_ends_of_its_range(tokens, scale):
+    """The largest and the least normal numbers, whose products are ordinary ones."""
+    x, w, t, gl = _case(tokens, 64, 300, F32)
+    _check(x * scale, w / scale, t, gl, F32)
+
+
+def test_xent_fp32_large_values_meet_large_gradients():
+    """A hidden state times its gradient's power of two is past fp32, the gradient of the weight is not."""
+    x, w, t, gl = _case(40, 64, 300, F32)
+    x, w = x * 1e30, w * 1e-30
+    x[3:] *= 1e-20  # those logits are 0 for any practical purpose
+    gl[0] = 1e12
+    ref = R.xent(x, w, t, -100, gl, out_dtype=F32)
+    _, lse = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    _, dw = mda.linear_cross_entropy_backward(gl.cuda(), x.cuda(), w.cuda(), t.cuda(), lse)
+    fits = ref["grad_weight"].abs() + ref["e_grad_weight"] < 3.4e38
+    assert bool(fits.any())
+    _close(torch.where(fits.cuda(), dw, torch.zeros_like(dw)), torch.where(fits, ref["grad_weight"], 0.0),
+           ref["e_grad_weight"], "grad_weight")
