@@ -12,10 +12,12 @@
 // softmax over columns reduces inside a lane.
 //
 // An operand of fp32 precision is two fp16 limbs of its values times a power of two that brings the
-// largest under 2^15 (x 2^s = hi + lo, 11 bits each, to 2^-22 of x, or 2^-40 of the largest where that
-// is more); a product of two of them is a list of segments, hi lo + lo hi + hi hi (lo lo is below
-// 2^-22), which the loop walks through as if k were three times as long, and a power of two undoes the
-// scales.  bf16 operands are one segment of bf16.  Accumulation is fp32 in the MFMA.
+// largest under 2^15: x 2^s = hi + 2^-11 lo.  fp16 holds 11 bits down to 2^-14 and steps of 2^-24 below; the low
+// limb is stored 2^11 up, so that it keeps its bits where hi has few left: x is off by 2^-22 of itself, or by
+// 2^-50 of the largest where that is more (with lo as it is: 2^-39).  A product of two of them is a list of
+// segments, hi lo + lo hi, then the accumulators times 2^-11, then hi hi (lo lo is below 2^-22), which the loop
+// walks through as if k were three times as long, and a power of two undoes the scales.  bf16 operands are
+// one segment of bf16.  Accumulation is fp32 in the MFMA.
 //
 // Tiles go to LDS by buffer_load_dwordx4 ... lds, NBUF - 1 to NBUF steps of 64 k ahead; rows and columns
 // past the end get an offset past the descriptor's range, which loads zeros.  16-byte chunks are
@@ -60,7 +62,8 @@ struct GemmArgs {
   int64_t ldpart;
   uint16_t* gb;          // g in bf16, or NULL
   float* delta;          // per compact token: what the target's g lacks
-  uint16_t* gh[2];       // g 2^(13 - e) in one or two fp16 limbs, 2^e the power of two below |gl|; or NULL
+  uint16_t* gh[2];       // g 2^(13 - e) in one or two fp16 limbs, 2^e the power of two below |gl|; or NULL.  Off by
+                         // 2^-12 of itself or 2^-38 of |gl|, two limbs: by 2^-22 or 2^-49
   int64_t ldg;
   float* slab;           // dX: [split][token][ldslab]
   int64_t ldslab, slab_stride;
@@ -204,6 +207,7 @@ __device__ __forceinline__ void tile_of(int id, int row_tiles, int col_tiles, in
   *ct = in / gr;
 }
 
+constexpr float kLowUp = 2048.0f;  // what the low limb of an operand is stored times
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 // compile-time loop: f(integral_constant 0), ..., f(N - 1)
@@ -327,7 +331,16 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
     each<TC + TR>([&](auto q) { read(0, q, lds, 0); });
   }
   uint32_t at = 0;
+  const int last_segment = steps - per_seg;
   for (int step = 0; step < steps; ++step) {
+    if constexpr (F16) {
+      if (step == last_segment && step > 0) {  // the segments before had one low limb each
+#pragma unroll
+        for (int i = 0; i < TC; ++i)
+#pragma unroll
+          for (int j = 0; j < TR; ++j) acc[i][j] *= 1.0f / kLowUp;
+      }
+    }
     const char* now = lds + at;
     at = at + kStage == NBUF * kStage ? 0 : at + kStage;
     const char* then = lds + at;
@@ -485,8 +498,8 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
           w[1] = pack_f16(v[2], v[3]);
           *reinterpret_cast<u32x2*>(a.gh[0] + to) = w;
           if (a.gh[1]) {
-            w[0] = pack_f16(v[0] - f16_lo(w[0]), v[1] - f16_hi(w[0]));
-            w[1] = pack_f16(v[2] - f16_lo(w[1]), v[3] - f16_hi(w[1]));
+            w[0] = pack_f16((v[0] - f16_lo(w[0])) * kLowUp, (v[1] - f16_hi(w[0])) * kLowUp);
+            w[1] = pack_f16((v[2] - f16_lo(w[1])) * kLowUp, (v[3] - f16_hi(w[1])) * kLowUp);
             *reinterpret_cast<u32x2*>(a.gh[1] + to) = w;
           }
         }

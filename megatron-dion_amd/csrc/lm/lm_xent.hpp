@@ -16,12 +16,14 @@
 //
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
 // whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, one
-// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs (2^-22) where the result is
+// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs where the result is
 // fp32: grad_weight into an fp32 main_grad (4096 tokens x 768 x 50257: 1.87 ms a pass, 2.34 with three
 // bf16 limbs; two bf16 limbs left 2.6e-6 of the 2-norm, twice what an fp32 product is off), and everything
 // for fp32 inputs, which are two fp16 limbs themselves.  The power of two that brings such an operand
 // into fp16's range comes from its largest finite value; g's is known, |p - [v = y]| <= 1 times the
 // mantissa of the token's gl, whose power of two goes into X (for dW) or is put back at the end (for dX).
+// Two limbs of g are off by 2^-22 of it or by 2^-49 of |gl|, whichever is more: a word's row keeps fp32's
+// bits down to p = 1e-8 and has 9 left at 1e-12; below 1e-15 it is 0.
 
 namespace xent {
 
@@ -220,8 +222,8 @@ __device__ __forceinline__ void pack8(const PackArgs& a, int64_t i, int rows, co
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         q[k] = pack_f16(v[2 * k], v[2 * k + 1]);
-        v[2 * k] -= f16_lo(q[k]);
-        v[2 * k + 1] -= f16_hi(q[k]);
+        v[2 * k] = (v[2 * k] - f16_lo(q[k])) * kLowUp;
+        v[2 * k + 1] = (v[2 * k + 1] - f16_hi(q[k])) * kLowUp;
       }
       *reinterpret_cast<u32x4*>(o) = q;
       o += static_cast<int64_t>(a.rows_p) * a.cols_p;

@@ -125,3 +125,61 @@ def test_xent_fp32_large_values_meet_large_gradients():
     assert bool(fits.any())
     _close(torch.where(fits.cuda(), dw, torch.zeros_like(dw)), torch.where(fits, ref["grad_weight"], 0.0),
            ref["e_grad_weight"], "grad_weight")
+
+
+def _spread_case(tokens, vocab, octaves, dtype):
+    """Logits without a rounding, from 0 down to -octaves log(2): column 0 of the hidden states is 1 and of the
+    weight the logit (multiples of 1/4), and the weight is 0 under the rest.  Targets are among the first 16
+    words, so that every other row of the weight's gradient is a sum of p gl x alone."""
+    x = _randn(1, tokens, 24, dtype=dtype)
+    x[:, 0] = 1.0
+    w = torch.zeros(vocab, 24)
+    w[:, 0] = -torch.floor(torch.arange(vocab) / (vocab - 1) * octaves * 0.693147 * 4) / 4
+    g = torch.Generator().manual_seed(2)
+    t = torch.randint(0, 16, (tokens,), generator=g)
+    return x, w.to(dtype), t, (0.5 + torch.rand(tokens, generator=g)) / tokens
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tokens", [30, 300, 2100])
+def test_xent_rows_of_rare_words_in_fp32_precision(dtype, tokens):
+    """The rows of words that are nobody's target, against their own size: g is off by 2^-21 of it or by 2^-48 of
+    gl, whichever is more (two fp16 limbs, the low one 2^11 up: each limb off by at most 2^-11 of itself or by
+    2^-25 of its unit, g at most 2^13 units)."""
+    vocab = 700
+    x, w, t, gl = _spread_case(tokens, vocab, 60, dtype)
+    xd, z = x.double(), x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse[:, None])
+    _, lse32 = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    _, dw = mda.linear_cross_entropy_backward(gl.cuda(), x.cuda(), w.cuda(), t.cuda(), lse32,
+                                              grad_weight=torch.empty(vocab, 24, device="cuda"))
+    g = p * gl.double()[:, None]
+    want = g.t() @ xd
+    # p: an exponent of up to 60 + log2(vocab) in fp32, two roundings of it, the lse's own error (a sum of 700
+    # terms in a tree and a logarithm: 64 roundings) and the exponential's; x: 2^-21 of it or 2^-48 of the largest
+    rel = (2 * 70 + 64 + 8) * R.U32 + 2.0 ** -21 + (2.0 ** -21 if dtype == F32 else 0.0)
+    off = rel * g + 2.0 ** -48 * gl.double()[:, None]
+    tol = off.t() @ xd.abs() + 3 * (tokens / 16 + 20) * R.U32 * (g.t() @ xd.abs())
+    tol = tol + (2.0 ** -48 * xd.abs().max() * g.sum(0)[:, None] if dtype == F32 else 0.0)
+    _close(dw[16:], want[16:], tol[16:], "grad_weight")
+    err = (dw.double().cpu() - want).norm(dim=1) / want.norm(dim=1)
+    common = p.amin(0) >= 1e-8
+    common[:16] = False
+    assert int(common.sum()) > 200 and float(err[common].max()) < 2e-5, float(err[common].max())
+
+
+def test_xent_small_values_of_fp32_inputs_keep_their_bits():
+    """Hidden states 2^-30 of the largest: each limb of X and W is off by at most 2^-11 of itself or by 2^-25 of
+    its unit, the largest at least 2^14 units and the low limb 2^11 up: 2^-21 of a value or 2^-49 of the largest."""
+    x, w, t, _ = _case(40, 64, 300, F32)
+    x[:20] *= 2.0 ** -30
+    w *= 2.0 ** 30
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]
+    loss, _ = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    size = (x.double().abs() @ w.double().abs().t()).amax(1)
+    ez = size * (3 * 2.0 ** -21 + 3 * (64 / 16 + 20) * R.U32) + 2.0 ** -49 * x.double().abs().max() * \
+        w.double().abs().sum(1).max()
+    tol = 2 * ez + (300 / 16 + 120) * R.U32 + 8 * R.U32 * z.abs().amax(1)
+    _close(loss[:20], want[:20], tol[:20], "loss")
