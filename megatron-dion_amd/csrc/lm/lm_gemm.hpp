@@ -60,10 +60,10 @@ struct GemmArgs {
   float2* part;          // stats: [part][token] (c, sum of 2^(x log2(e) - c))
   float* tlogit;         // stats: per compact token
   int64_t ldpart;
-  uint16_t* gb;          // g in bf16, or NULL
+  uint16_t* gb[2];       // g in bf16 and what that lacks in another, each or both NULL
   float* delta;          // per compact token: what the target's g lacks
-  uint16_t* gh[2];       // g 2^(13 - e) in one or two fp16 limbs, 2^e the power of two below |gl|; or NULL.  Off by
-                         // 2^-12 of itself or 2^-38 of |gl|, two limbs: by 2^-22 or 2^-49
+  uint16_t* gh[2];       // g 2^(13 - e) in two fp16 limbs, 2^e the power of two below |gl|, or NULL: off by
+                         // 2^-22 of itself or 2^-49 of |gl|
   int64_t ldg;
   float* slab;           // dX: [split][token][ldslab]
   int64_t ldslab, slab_stride;
@@ -476,17 +476,24 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
       if constexpr (EPI == EPI_GRAD) {
         const int64_t to = static_cast<int64_t>(orow) * a.ldg + col;
         const float glr = __shfl(gl, rr, 64);  // lane rr has row rr's
-        if (a.gb) {
+        if (a.gb[0]) {
           f32x4 u = v * glr;
           u32x2 w;
           w[0] = pack_bf16(u[0], u[1]);
           w[1] = pack_bf16(u[2], u[3]);
-          *reinterpret_cast<u32x2*>(a.gb + to) = w;
-          if (here) {
+          *reinterpret_cast<u32x2*>(a.gb[0] + to) = w;
+          if (here || a.gb[1]) {
             u[0] -= __uint_as_float(w[0] << 16);
             u[1] -= __uint_as_float(w[0] & 0xFFFF0000u);
             u[2] -= __uint_as_float(w[1] << 16);
             u[3] -= __uint_as_float(w[1] & 0xFFFF0000u);
+          }
+          if (a.gb[1]) {
+            w[0] = pack_bf16(u[0], u[1]);
+            w[1] = pack_bf16(u[2], u[3]);
+            *reinterpret_cast<u32x2*>(a.gb[1] + to) = w;
+          }
+          if (here) {
             const int at = __shfl(tgt, rr, 64) - 4 * c;
             if (orow < n_valid && at >= 0 && at < 4) a.delta[orow] = at == 0 ? u[0] : at == 1 ? u[1] : at == 2 ? u[2] : u[3];
           }
@@ -497,11 +504,9 @@ __global__ void __launch_bounds__(64 * (BR / WR) * (BC / WC)) gemm_kernel(const 
           w[0] = pack_f16(v[0], v[1]);
           w[1] = pack_f16(v[2], v[3]);
           *reinterpret_cast<u32x2*>(a.gh[0] + to) = w;
-          if (a.gh[1]) {
-            w[0] = pack_f16((v[0] - f16_lo(w[0])) * kLowUp, (v[1] - f16_hi(w[0])) * kLowUp);
-            w[1] = pack_f16((v[2] - f16_lo(w[1])) * kLowUp, (v[3] - f16_hi(w[1])) * kLowUp);
-            *reinterpret_cast<u32x2*>(a.gh[1] + to) = w;
-          }
+          w[0] = pack_f16((v[0] - f16_lo(w[0])) * kLowUp, (v[1] - f16_hi(w[0])) * kLowUp);
+          w[1] = pack_f16((v[2] - f16_lo(w[1])) * kLowUp, (v[3] - f16_hi(w[1])) * kLowUp);
+          *reinterpret_cast<u32x2*>(a.gh[1] + to) = w;
         }
       } else if constexpr (EPI == EPI_SLAB) {
         if (orow < n_valid && col < a.ldslab) {

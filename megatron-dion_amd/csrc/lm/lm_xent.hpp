@@ -15,8 +15,9 @@
 // holds is never read.
 //
 // Precision: bf16 inputs are multiplied as they are.  g is one bf16 (2^-8) where it makes bf16 results,
-// whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, one
-// fp16 limb, 2^-11: that product is bound by writing dW), and two fp16 limbs where the result is
+// whose own rounding is as large (for dW of up to 256 tokens, where few roundings do not average out, two
+// bf16, 2^-16 over bf16's whole range.  One fp16 limb, 2^-11, is 0 below p = 4e-12; gradients of 8 / 256
+// tokens x 4096 x 32000 take 263 / 377 us with it, 268 / 418 with two bf16), and two fp16 limbs where the result is
 // fp32: grad_weight into an fp32 main_grad (4096 tokens x 768 x 50257: 1.87 ms a pass, 2.34 with three
 // bf16 limbs; two bf16 limbs left 2.6e-6 of the 2-norm, twice what an fp32 product is off), and everything
 // for fp32 inputs, which are two fp16 limbs themselves.  The power of two that brings such an operand
@@ -387,10 +388,10 @@ __global__ void __launch_bounds__(256) round_kernel(const float* slab, int split
 // ------------------------------------------------------------------------------- plan
 struct Plan {
   int f32;             // fp32 inputs
-  int wide;            // backward: grad_weight in fp32 precision
+  int wide;            // backward: grad_weight in fp32 precision, from two fp16 limbs of g
   int limbs_in;        // of X and W
-  int dw_limbs;        // backward: fp16 limbs of g for dW, 0: its bf16
-  int g_arrays;        // backward: 16-bit arrays of g: the bf16 (bf16 inputs), then the limbs
+  int g_bf16;          // backward: bf16 of g (bf16 inputs): one, or two for dW of few tokens
+  int g_arrays;        // backward: 16-bit arrays of g: the bf16, then the fp16 limbs
   int logits, dx;      // tiles of the products (kTiles); dW's goes by the piece
   int tokens_p, hidden_p;
   bool pack_w;
@@ -440,8 +441,8 @@ Plan make_plan(const DionXentDesc* d, int op) {
   p.f32 = d->dtype == DION_DTYPE_F32;
   p.wide = op == DION_XENT_BACKWARD && (p.f32 || d->gw_dtype == DION_DTYPE_F32);
   p.limbs_in = p.f32 ? 2 : 1;
-  p.dw_limbs = p.wide ? 2 : op == DION_XENT_BACKWARD && d->tokens <= 256 ? 1 : 0;
-  p.g_arrays = (p.f32 ? 0 : 1) + p.dw_limbs;
+  p.g_bf16 = p.f32 ? 0 : !p.wide && d->tokens <= 256 ? 2 : 1;
+  p.g_arrays = p.g_bf16 + (p.wide ? 2 : 0);
   p.logits = pick_tile(d->tokens, d->vocab, 1, 3);
   p.dx = pick_tile(d->tokens, d->hidden, ceil_div(d->vocab, 256), d->tokens >= 256 ? 3 : d->tokens > 64 ? 2 : 1);
   const int br = kTiles[p.logits].br > kTiles[p.dx].br ? kTiles[p.logits].br : kTiles[p.dx].br;
@@ -475,8 +476,8 @@ Plan make_plan(const DionXentDesc* d, int op) {
   const size_t tp = static_cast<size_t>(p.tokens_p);
   p.tok = take(512 + 3 * kAmaxBlocks * sizeof(float) + 7 * tp * 4);
   p.xp = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
-  if (p.dw_limbs) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
-  if (p.f32 || p.dw_limbs) {
+  if (p.wide) p.xg = take(static_cast<size_t>(p.limbs_in) * tp * p.hidden_p * 2);
+  if (p.f32 || p.wide) {
     const long units = (d->tokens + (p.f32 ? d->vocab : 0)) * ceil_div(d->hidden, 8);
     p.amax_blocks = static_cast<int>(units > kAmaxBlocks * 1024L ? kAmaxBlocks : ceil_div(units, 1024));
   }
@@ -625,7 +626,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
     m.vocab = d->vocab;
     m.hidden = d->hidden;
     m.want_x = m.want_w = p.f32;
-    m.want_xg = p.dw_limbs > 0;
+    m.want_xg = p.wide;
     m.target = target;
     m.gl = gl;
     m.ignore = d->ignore_index;
@@ -641,7 +642,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   memset(&xg, 0, sizeof(xg));
   memset(&w, 0, sizeof(w));
   xg.cols_p = w.cols_p = 8;
-  if (p.dw_limbs) {
+  if (p.wide) {
     xg = x;
     xg.dst = reinterpret_cast<uint16_t*>(ws + p.xg);
     xg.f16 = 1;
@@ -661,7 +662,7 @@ int prepare(const DionXentDesc* d, const Plan& p, const void* hidden, const void
   hipLaunchKernelGGL(select_kernel, dim3(1), dim3(1024), 0, st, a, p.amax_blocks);
   int rc = check_launch("xent(select)");
   if (rc == DION_OK) rc = pack(x, tok, p, st, "xent(pack hidden)");
-  if (rc == DION_OK && p.dw_limbs) rc = pack(xg, tok, p, st, "xent(pack hidden for dW)");
+  if (rc == DION_OK && p.wide) rc = pack(xg, tok, p, st, "xent(pack hidden for dW)");
   if (rc == DION_OK && p.pack_w) rc = pack(w, tok, p, st, "xent(pack weight)");
   return rc;
 }
@@ -756,12 +757,10 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     logits_args(&a, d, p, x, w, ldw, stride, v0, n, tok);
     a.lse = tok.lse;
     a.gl = tok.gl;
-    uint16_t* wide = p.f32 ? g : g + gstride;  // the fp16 limbs
-    if (!p.f32) {
-      a.gb = g;
-      a.delta = tok.delta;
-    }
-    for (int l = 0; l < p.dw_limbs; ++l) a.gh[l] = wide + l * gstride;
+    uint16_t* limbs = g + p.g_bf16 * gstride;  // fp16
+    for (int l = 0; l < p.g_bf16; ++l) a.gb[l] = g + l * gstride;
+    if (p.g_bf16) a.delta = tok.delta;
+    for (int l = 0; p.wide && l < 2; ++l) a.gh[l] = limbs + l * gstride;
     a.ldg = p.piece;
     rc = launch<false, false, EPI_GRAD>(p.f32, p.logits, a, p.tokens_p, n, st, "xent(logit gradients)");
     if (rc != DION_OK) return rc;
@@ -784,9 +783,9 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
     }
     if (grad_weight) {
       memset(&a, 0, sizeof(a));
-      if (p.dw_limbs) segments(&a, wide, gstride, p.dw_limbs, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
-      else segments(&a, g, gstride, 1, x, xstride, 1);
-      a.scale = p.dw_limbs ? tok.scale + kScaleDw : nullptr;
+      if (p.wide) segments(&a, limbs, gstride, 2, reinterpret_cast<uint16_t*>(ws + p.xg), xstride, p.limbs_in);
+      else segments(&a, g, gstride, p.g_bf16, x, xstride, 1);
+      a.scale = p.wide ? tok.scale + kScaleDw : nullptr;
       a.ldr = p.piece;
       a.ldc = p.hidden_p;
       a.cols = d->hidden;
@@ -802,7 +801,7 @@ int backward(const DionXentDesc* d, const void* hidden, const void* weight, cons
       // tiles stay inside the piece of g (a multiple of 256 words): what lies past n there makes rows
       // that are not stored
       const int tile = pick_tile(n, d->hidden, 1, d->tokens >= 512 ? 3 : 2);
-      rc = launch<true, true, EPI_OUT>(p.dw_limbs > 0, tile, a, n, d->hidden, st, "xent(grad weight)");
+      rc = launch<true, true, EPI_OUT>(p.wide, tile, a, n, d->hidden, st, "xent(grad weight)");
       if (rc != DION_OK) return rc;
     }
   }

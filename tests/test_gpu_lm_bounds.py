@@ -183,3 +183,19 @@ def test_xent_small_values_of_fp32_inputs_keep_their_bits():
         w.double().abs().sum(1).max()
     tol = 2 * ez + (300 / 16 + 120) * R.U32 + 8 * R.U32 * z.abs().amax(1)
     _close(loss[:20], want[:20], tol[:20], "loss")
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 256, 300])
+def test_xent_bf16_rows_of_rare_words(tokens):
+    """bf16 gradients of words down to p = 2^-100, few tokens or many: bf16 has fp32's range, and so has g."""
+    vocab = 700
+    x, w, t, gl = _spread_case(tokens, vocab, 100, BF16)
+    xd, z = x.double(), x.double() @ w.double().t()
+    p = torch.softmax(z, 1)
+    _, lse32 = mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda())
+    _, dw = mda.linear_cross_entropy_backward(gl.cuda(), x.cuda(), w.cuda(), t.cuda(), lse32)
+    g = p * gl.double()[:, None]
+    want, size = g.t() @ xd, g.t() @ xd.abs()
+    # p as above with exponents of 110; g: one bf16 (2^-8), of up to 256 tokens two (2^-16)
+    rel = (2 * 110 + 64 + 8) * R.U32 + (2.0 ** -8 if tokens > 256 else 2.0 ** -16) + (tokens / 16 + 20) * 2 * R.U32
+    _close(dw[16:], want[16:], rel * size[16:] + R.half_step(BF16) * want[16:].abs(), "grad_weight")
