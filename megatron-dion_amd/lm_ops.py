@@ -291,6 +291,7 @@ def _xent_shape(op, tokens, hidden, vocab, dtype, gw_dtype, accumulate, pack_wei
 
 def _xent_desc(op, hidden, weight, target, vocab_start, vocab_size, ignore_index, grad_weight=None, accumulate=False,
                piece_bytes=0):
+    """The descriptor and scratch of a call, None if the weight holds no word of the vocabulary."""
     tokens, cols, ld_h = _rows(hidden, "hidden")
     if weight.dim() != 2 or weight.shape[1] != cols or weight.dtype != hidden.dtype or weight.device != hidden.device:
         raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] hidden {tuple(hidden.shape)} {hidden.dtype} {hidden.device}, "
@@ -302,12 +303,14 @@ def _xent_desc(op, hidden, weight, target, vocab_start, vocab_size, ignore_index
     code = _dtype(hidden, "hidden")
     start = int(vocab_start)
     total = start + rows if vocab_size is None else int(vocab_size)
-    if start < 0 or rows < 1 or total <= start:
+    if start < 0 or total < 1:
         raise RuntimeError(f"[DION_BAD_VOCAB] weight of {rows} rows from word {start} on, of {total}")
     vocab = min(rows, total - start)  # rows past the vocabulary are padding
     gw_code, ld_gw = code, cols
     if grad_weight is not None:
         gw_code, ld_gw = _dtype(grad_weight, "grad_weight"), _rows(grad_weight, "grad_weight")[2]
+    if vocab < 1:
+        return None, 0
     return _xent_shape(op, tokens, cols, vocab, code, gw_code, int(bool(accumulate)), int(weight.data_ptr() % 16 != 0),
                        start, total, int(ignore_index), ld_h, ld_w, ld_gw, int(piece_bytes))
 
@@ -324,6 +327,13 @@ def combine_vocab_shards(lse: torch.Tensor, tlogit: torch.Tensor, ignored: torch
     return torch.where(ignored, torch.zeros_like(top), lse - both[1]), lse
 
 
+def _sum_over_shards(grad_hidden: Optional[torch.Tensor], group) -> Optional[torch.Tensor]:
+    if group is not None and grad_hidden is not None:
+        with torch.cuda.device(grad_hidden.device):
+            dist.all_reduce(grad_hidden, op=dist.ReduceOp.SUM, group=group)
+    return grad_hidden
+
+
 def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,
                                  vocab_start: int = 0, vocab_size: Optional[int] = None, ignore_index: int = -100,
                                  group=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -337,11 +347,20 @@ def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, tar
 
     Vocabulary shards (tensor parallel): weight holds the rows from `vocab_start` on of a vocabulary of
     `vocab_size` words (rows past it are padding), `group` the ranks that share it; every rank passes the
-    same hidden states and targets and gets the whole vocabulary's loss."""
+    same hidden states and targets and gets the whole vocabulary's loss.  A rank all of whose rows are
+    padding takes part as the others do."""
     if group is not None and vocab_size is None:
         raise RuntimeError("[DION_BAD_VOCAB] a vocabulary in shards needs vocab_size, the words of all of them")
     d, nbytes = _xent_desc(_lm_lib.XENT_FORWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index)
     device = hidden.device
+    if d is None:
+        if group is None:
+            raise RuntimeError(f"[DION_BAD_VOCAB] no word of {vocab_size} in weight of {weight.shape[0]} rows from "
+                               f"word {int(vocab_start)} on")
+        # the other ranks of the group wait in its reductions
+        lse = torch.full(target.shape, float("-inf"), dtype=torch.float32, device=device)
+        with torch.cuda.device(device):
+            return combine_vocab_shards(lse, torch.zeros_like(lse), target == ignore_index, group)
     target = target.contiguous()
     ws = _workspace(nbytes, device)
     loss = torch.empty(target.shape, dtype=torch.float32, device=device)
@@ -385,10 +404,13 @@ def linear_cross_entropy_backward(grad_loss: torch.Tensor, hidden: torch.Tensor,
             raise RuntimeError(f"[DION_INCONSISTENT_TENSORS] {what}: fp32 {tuple(target.shape)} expected, got "
                                f"{t.dtype} {tuple(t.shape)} {t.device}")
     gh = _empty(hidden) if need_hidden else None
-    if gw is not None and not accumulate and (d.tokens == 0 or d.vocab < weight.shape[0]):
-        (gw if d.tokens == 0 else gw[d.vocab:]).zero_()
-    if d.tokens == 0 or (gh is None and gw is None):
-        return gh, gw
+    none = d is None or d.tokens == 0  # no gradient: of no word, or no token's
+    if gw is not None and not accumulate and (none or d.vocab < weight.shape[0]):
+        (gw if none else gw[d.vocab:]).zero_()
+    if none and gh is not None:
+        gh.zero_()
+    if none or (gh is None and gw is None):
+        return _sum_over_shards(gh, group), gw
     target, grad_loss, lse = target.contiguous(), grad_loss.contiguous(), lse.contiguous()
     ws = _workspace(nbytes, device)
     rc = _call(_lm_lib.load().dion_xent_backward, device, _byref(d), hidden.data_ptr(), weight.data_ptr(),
@@ -396,7 +418,4 @@ def linear_cross_entropy_backward(grad_loss: torch.Tensor, hidden: torch.Tensor,
                None if gw is None else gw.data_ptr(), ws.data_ptr(), ws.numel())
     if rc:
         _lm_lib.check(rc, "dion_xent_backward")
-    if group is not None and gh is not None:
-        with torch.cuda.device(device):
-            dist.all_reduce(gh, op=dist.ReduceOp.SUM, group=group)
-    return gh, gw
+    return _sum_over_shards(gh, group), gw
