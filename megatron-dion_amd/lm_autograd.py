@@ -33,13 +33,20 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else t.contiguous()
 
 
+def _main_grad(weight: torch.Tensor) -> torch.Tensor:
+    main = getattr(weight, "main_grad", None)
+    if main is None:
+        raise RuntimeError("[DION_NO_MAIN_GRAD] into_main_grad: weight has no main_grad")
+    return main
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, target, kwargs, main_grad):
+    def forward(ctx, hidden, weight, target, kwargs, owner):
         _eager("linear_cross_entropy")
         loss, lse = lm_ops.linear_cross_entropy_forward(hidden, weight, target, **kwargs)
         ctx.save_for_backward(hidden, weight, target, lse)
-        ctx.kwargs, ctx.main_grad = kwargs, main_grad
+        ctx.kwargs, ctx.owner = kwargs, owner
         return loss
 
     @staticmethod
@@ -48,10 +55,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
         _eager("linear_cross_entropy")
         hidden, weight, target, lse = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
+        # the owner's main_grad of now: the optimizer may have been given another buffer since the forward pass
+        main = _main_grad(ctx.owner) if need_w and ctx.owner is not None else None
         gh, gw = lm_ops.linear_cross_entropy_backward(
-            _rows(grad_loss), hidden, weight, target, lse, grad_weight=ctx.main_grad if need_w else None,
-            accumulate=need_w and ctx.main_grad is not None, need_hidden=need_h, need_weight=need_w, **ctx.kwargs)
-        return gh, None if ctx.main_grad is not None else gw, None, None, None
+            _rows(grad_loss), hidden, weight, target, lse, grad_weight=main, accumulate=main is not None,
+            need_hidden=need_h, need_weight=need_w, **ctx.kwargs)
+        return gh, None if main is not None else gw, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, vocab_start: int = 0,
@@ -60,13 +69,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     """Each token's cross entropy of `hidden @ weight.T` (fp32, target's shape), differentiable in hidden
     and weight.  `into_main_grad`: the backward pass adds weight's gradient to `weight.main_grad`, where
     the optimizer reads it, and leaves `weight.grad` (and its hooks) alone."""
-    main = None
     if into_main_grad:
-        main = getattr(weight, "main_grad", None)
-        if main is None:
-            raise RuntimeError("[DION_NO_MAIN_GRAD] into_main_grad: weight has no main_grad")
+        _main_grad(weight)
     kwargs = dict(vocab_start=vocab_start, vocab_size=vocab_size, ignore_index=ignore_index, group=group)
-    return _LinearCrossEntropy.apply(hidden, weight, target, kwargs, main)
+    return _LinearCrossEntropy.apply(hidden, weight, target, kwargs, weight if into_main_grad else None)
 
 
 class _RmsNormAdd(torch.autograd.Function):
