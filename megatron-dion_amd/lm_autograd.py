@@ -40,6 +40,14 @@ def _main_grad(weight: torch.Tensor) -> torch.Tensor:
     return main
 
 
+def _backward_waits_for(device: torch.device) -> None:
+    """The caller of backward() finds main_grad written: autograd joins the streams of the gradients that it
+    hands on, and this one it does not know."""
+    done = torch.cuda.current_stream(device).record_event()
+    torch.autograd.Variable._execution_engine.queue_callback(
+        lambda: torch.cuda.current_stream(device).wait_event(done))
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, kwargs, owner):
@@ -60,6 +68,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         gh, gw = lm_ops.linear_cross_entropy_backward(
             _rows(grad_loss), hidden, weight, target, lse, grad_weight=main, accumulate=main is not None,
             need_hidden=need_h, need_weight=need_w, **ctx.kwargs)
+        if main is not None:
+            _backward_waits_for(main.device)
         return gh, None if main is not None else gw, None, None, None
 
 

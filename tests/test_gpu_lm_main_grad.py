@@ -42,3 +42,23 @@ def test_loss_of_a_frozen_weight_leaves_its_main_grad():
     xg = x.clone().requires_grad_()
     mda.linear_cross_entropy(xg, w, t, into_main_grad=True).sum().backward()
     assert (w.main_grad == 0).all() and xg.grad.abs().sum() > 0
+
+
+@pytest.mark.parametrize("used_before", [False, True])
+def test_loss_on_another_stream_into_main_grad(used_before):
+    """Forward on a side stream that is behind, backward from the default stream, which reads main_grad next."""
+    x, w, t, want = _loss_case()
+    w.main_grad = torch.zeros_like(w)
+    other = w.sum() if used_before else 0.0  # the parameter's own node belongs to the default stream then
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = mda.linear_cross_entropy(x, w, t, into_main_grad=True)
+    torch.cuda.current_stream().wait_stream(side)
+    total = loss.sum() + other
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)
+    total.backward()
+    got = w.main_grad.clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
