@@ -77,8 +77,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
                          vocab_size: Optional[int] = None, ignore_index: int = -100, group=None,
                          into_main_grad: bool = False) -> torch.Tensor:
     """Each token's cross entropy of `hidden @ weight.T` (fp32, target's shape), differentiable in hidden
-    and weight.  `into_main_grad`: the backward pass adds weight's gradient to `weight.main_grad`, where
-    the optimizer reads it, and leaves `weight.grad` (and its hooks) alone."""
+    and weight.  `into_main_grad`: the backward pass adds weight's gradient to the `weight.main_grad` it finds,
+    where the optimizer reads it, on the stream of the forward pass, and leaves `weight.grad` and the
+    parameter's hooks alone: what waits for such a hook (an overlapped gradient reduction) has to be told
+    otherwise."""
     if into_main_grad:
         _main_grad(weight)
     kwargs = dict(vocab_start=vocab_start, vocab_size=vocab_size, ignore_index=ignore_index, group=group)
@@ -87,11 +89,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
 
 class _RmsNormAdd(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps, p, rng):
+    def forward(ctx, x, weight, residual, eps, p, rng, owner):
         _eager("rms_norm_add")
         f = lm_ops.rms_norm_add_forward(x, weight, residual, eps=eps, p=p, rng=rng)
         ctx.save_for_backward(f.h, weight, f.rstd)
-        ctx.p, ctx.rng, ctx.stored = p, _held(rng), f.h is not x
+        ctx.p, ctx.rng, ctx.stored, ctx.owner = p, _held(rng), f.h is not x, owner
         ctx.set_materialize_grads(False)
         return (f.y, f.h) if ctx.stored else f.y
 
@@ -102,21 +104,30 @@ class _RmsNormAdd(torch.autograd.Function):
         h, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if grad_y is None and grad_h is None:
-            return (None,) * 6
+            return (None,) * 7
         if grad_y is None:  # only the residual stream was used
             g = _rows(grad_h)
             gx = lm_ops.dropout_add_backward(g, p=ctx.p, rng=ctx.rng) if need_x and ctx.p > 0.0 else g
-            return gx if need_x else None, None, g if need_r else None, None, None, None
+            return gx if need_x else None, None, g if need_r else None, None, None, None, None
+        main = _main_grad(ctx.owner) if need_w and ctx.owner is not None else None
         b = lm_ops.rms_norm_add_backward(_rows(grad_y), h, weight, rstd, _rows(grad_h), p=ctx.p, rng=ctx.rng,
+                                         grad_weight=main, accumulate=main is not None,
                                          need_input=need_x or need_r, need_weight=need_w, need_residual=need_r)
-        return b.grad_x if need_x else None, b.grad_weight, b.grad_residual if need_r else None, None, None, None
+        if main is not None:
+            _backward_waits_for(main.device)
+        return (b.grad_x if need_x else None, None if main is not None else b.grad_weight,
+                b.grad_residual if need_r else None, None, None, None, None)
 
 
 def rms_norm_add(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
-                 eps: float = 1e-5, p: float = 0.0, rng: Optional[lm_ops.Rng] = None
+                 eps: float = 1e-5, p: float = 0.0, rng: Optional[lm_ops.Rng] = None, into_main_grad: bool = False
                  ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(y, h): `h = residual + dropout(x)` and its RMS norm, differentiable in x, weight and residual."""
-    out = _RmsNormAdd.apply(x, weight, residual, eps, p, rng)
+    """(y, h): `h = residual + dropout(x)` and its RMS norm, differentiable in x, weight and residual.
+    `into_main_grad` as in `linear_cross_entropy`.  The 8-bit output has no form here: nothing
+    differentiates it, and the explicit calls give it with its gradients."""
+    if into_main_grad:
+        _main_grad(weight)
+    out = _RmsNormAdd.apply(x, weight, residual, eps, p, rng, weight if into_main_grad else None)
     return out if isinstance(out, tuple) else (out, x)
 
 

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import megatron_dion_amd as mda
+from megatron_dion_amd.optimizer import attach_dp_routing
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +63,33 @@ def test_loss_on_another_stream_into_main_grad(used_before):
     got = w.main_grad.clone()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,main_dtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_norm_adds_to_main_grad(dtype, main_dtype, p):
+    g = torch.Generator().manual_seed(5)
+    x, r, gy = (torch.randn(33, 72, generator=g).to(dtype).cuda() for _ in range(3))
+    w = torch.nn.Parameter((1 + 0.2 * torch.randn(72, generator=g)).cuda())
+    rng = (3, 4) if p else None
+    f = mda.rms_norm_add_forward(x, w.detach(), r, p=p, rng=rng)
+    b = mda.rms_norm_add_backward(gy, f.h, w.detach(), f.rstd, None, p=p, rng=rng,
+                                  grad_weight=torch.zeros(72, dtype=main_dtype, device="cuda"))
+    xg, rg = x.clone().requires_grad_(), r.clone().requires_grad_()
+    before = w.main_grad = torch.zeros(72, dtype=main_dtype, device="cuda")
+    y, _ = mda.rms_norm_add(xg, w, rg, p=p, rng=rng, into_main_grad=True)
+    w.main_grad = torch.zeros(72, dtype=main_dtype, device="cuda")
+    y.backward(gy)
+    assert torch.equal(w.main_grad, b.grad_weight) and (before == 0).all() and w.grad is None
+    assert torch.equal(xg.grad, b.grad_x) and torch.equal(rg.grad, b.grad_residual)
+    y, h = mda.rms_norm_add(xg, w, rg, p=p, rng=rng, into_main_grad=True)
+    h.sum().backward()  # only the residual stream: nothing for the weight
+    assert torch.equal(w.main_grad, b.grad_weight)
+    opt = mda.MegatronDion([w], lr=0.01)
+    attach_dp_routing(opt, [("norm.weight", w)])
+    w0 = w.detach().clone()
+    opt.step()
+    assert torch.isfinite(w).all() and not torch.equal(w.detach(), w0)
+    del w.main_grad
+    with pytest.raises(RuntimeError, match="DION_NO_MAIN_GRAD"):
+        mda.rms_norm_add(xg, w, rg, p=p, rng=rng, into_main_grad=True)
