@@ -199,3 +199,24 @@ def test_xent_bf16_rows_of_rare_words(tokens):
     # p as above with exponents of 110; g: one bf16 (2^-8), of up to 256 tokens two (2^-16)
     rel = (2 * 110 + 64 + 8) * R.U32 + (2.0 ** -8 if tokens > 256 else 2.0 ** -16) + (tokens / 16 + 20) * 2 * R.U32
     _close(dw[16:], want[16:], rel * size[16:] + R.half_step(BF16) * want[16:].abs(), "grad_weight")
+
+
+# ------------------------------------------------------------------------------- dropout
+def test_dropout_past_the_low_word_of_the_group():
+    """2^34 + 4096 elements: groups of four from 2^32 on have a second counter word that is not 0."""
+    n, seed, offset = (1 << 34) + 4096, 11, 13
+    x = torch.ones(n, dtype=BF16, device="cuda")
+    out = mda.dropout_add_forward(x, p=0.5, rng=(seed, offset))
+    m32 = 0xFFFFFFFF
+    want = []
+    for group in range((1 << 32) - 256, (1 << 32) + 1024):
+        c, k = [group & m32, group >> 32, offset, 0], [seed, 0]
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & m32, (a >> 32) ^ c[3] ^ k[1], a & m32]
+            k = [(k[0] + 0x9E3779B9) & m32, (k[1] + 0xBB67AE85) & m32]
+        want += [word >= 1 << 31 for word in c]
+    assert (out[(1 << 34) - 1024:].cpu() != 0).tolist() == want
+    first = R.keep_mask((4096,), 0.5, seed, offset)
+    assert torch.equal(out[:4096].cpu() != 0, first)
+    assert not torch.equal(out[1 << 34:].cpu() != 0, first)
