@@ -69,7 +69,7 @@ typedef struct DionNormDesc {
   int32_t w_dtype;     /* weight: F32 or BF16                                                 */
   int32_t gw_dtype;    /* grad_weight: F32 or BF16                                            */
   int32_t y_dtype;     /* `dtype`, or E4M3 (8 bits with scales)                               */
-  int32_t scale_block; /* E4M3: columns that share a scale, 1 .. cols (cols: one a row)       */
+  int32_t scale_block; /* E4M3: columns that share a scale, min(8, cols) .. cols (cols: one a row) */
   int32_t accumulate;  /* backward: grad_weight += instead of =                               */
   float eps;
   double p;            /* dropout of x, 0 <= p <= 1                                           */

@@ -9,7 +9,7 @@ import ctypes
 import hashlib
 import os
 
-from ._lib import DTYPE_BF16, DTYPE_F32, DionLibraryError, DionUnsupportedError, DION_E_UNSUPPORTED, DION_OK
+from ._lib import DionLibraryError, DionUnsupportedError, DION_E_UNSUPPORTED, DION_OK
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "csrc", "libdion_lm.so")
@@ -131,6 +131,3 @@ def check(rc: int, what: str) -> None:
         err = cls(f"[DION_HIP_ERROR] {what} failed ({rc}): {msg}")
         err.code = rc
         raise err
-
-
-DTYPES = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}

@@ -418,8 +418,10 @@ struct TileShape {
 };
 constexpr TileShape kTiles[4] = {{64, 64, 32}, {64, 128, 64}, {128, 128, 64}, {256, 256, 128}};
 
-// The largest tile that makes `parts` x `rows` x `cols` into enough blocks for 256 CUs, and that the rows
-// fill.  Measured (us, tile 256 / 128 / 64x128 / 64; blocks of the first):
+// The largest tile, up to `most`, that makes `parts` x `rows` x `cols` into enough blocks for 256 CUs.  The
+// tokens bound `most` for dX and dW, but not for the logits: under more than 32640 words a few tokens take
+// tiles of 128 rows, from 48897 on of 256, most of them zeros: the logits' last line has what that
+// costs.  Measured (us, tile 256 / 128 / 64x128 / 64; blocks of the first):
 //   logits   8192 tokens x 32000 words, h 4096: 907 (2000 blocks) / 1074 / 1470 / 1767 at 4096 tokens;
 //            122 (250) / 148 / 188 / 222 at 512;  106 (125) / 78 / 102 / 114 at 256;
 //            91 / 60 / 55 / 68 at 128;  89 / 58 / 49 / 54 at 1
@@ -535,7 +537,9 @@ int launch_as(int tile, const GemmArgs& a, long rows, long cols, hipStream_t st,
     case 1:
       // The loss of up to 64 tokens alone: W passes by once, non-temporal.  One token under 32000 words of
       // 4096: 60.2 us against 64.5 where a gigabyte of other weights has been read since, 63.7 against 48.1
-      // where the last-level cache still holds W.  The backward pass reads W twice and keeps it.
+      // where the last-level cache still holds W.  The tokens alone choose it: a weight that the cache holds
+      // from one call to the next pays, and so do limbs in the workspace, which the call has just written (fp32
+      // reads the high one twice).  The backward pass reads W twice and keeps it.
       if constexpr (EPI == EPI_STATS)
         if (rows <= 64) return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3, true>(a, rows, cols, st, what);
       return launch_tile<64, 128, 32, 64, RKS, CKS, F16, EPI, 3>(a, rows, cols, st, what);

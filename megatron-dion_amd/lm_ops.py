@@ -2,16 +2,16 @@
 
 The optimizer consumes gradients; these make those of the parameters its elementwise branch updates
 (the output layer and the norms), in hand-written HIP kernels (csrc/lm/, C ABI in include/dion_lm.h).
-They take the place of what a Megatron model calls there: the vocabulary-parallel cross entropy after
-its output layer, the bias-dropout-add before a norm, and the norm itself.
+They take the place of what a Megatron model without biases calls there: the vocabulary-parallel cross
+entropy after its output layer, the dropout-add before a norm, and the norm itself.
 
 Each operator is a pair of explicit calls, forward and backward, that run on the current HIP stream of
 the tensors' device, allocate their results and scratch from torch's caching allocator, never wait for
 the GPU and can be captured into a graph.  `lm_autograd.py` wraps them for autograd.
 
-Tensors are float32 or bfloat16 of any leading shape, with unit stride along the last axis and the
-leading axes evenly strided (what `view(-1, cols)` accepts); anything else raises
-``RuntimeError("[DION_...] ...")`` before any work is enqueued.
+Tensors are float32 or bfloat16 of any leading shape, with unit stride along the last axis, the
+leading axes evenly strided and rows that do not overlap (an expanded axis is refused); anything else
+raises ``RuntimeError("[DION_...] ...")`` before any work is enqueued.
 """
 from __future__ import annotations
 
