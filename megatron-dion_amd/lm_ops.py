@@ -348,15 +348,15 @@ def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, tar
     Vocabulary shards (tensor parallel): weight holds the rows from `vocab_start` on of a vocabulary of
     `vocab_size` words (rows past it are padding), `group` the ranks that share it; every rank passes the
     same hidden states and targets and gets the whole vocabulary's loss.  A rank all of whose rows are
-    padding takes part as the others do."""
+    padding takes part as the others do.  A shard without `group` is refused: it has no loss."""
     if group is not None and vocab_size is None:
         raise RuntimeError("[DION_BAD_VOCAB] a vocabulary in shards needs vocab_size, the words of all of them")
     d, nbytes = _xent_desc(_lm_lib.XENT_FORWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index)
     device = hidden.device
+    if group is None and (d is None or d.vocab < d.vocab_total):
+        raise RuntimeError(f"[DION_BAD_VOCAB] weight of {weight.shape[0]} rows from word {int(vocab_start)} on holds a "
+                           "part of the vocabulary: its loss needs group")
     if d is None:
-        if group is None:
-            raise RuntimeError(f"[DION_BAD_VOCAB] no word of {vocab_size} in weight of {weight.shape[0]} rows from "
-                               f"word {int(vocab_start)} on")
         # the other ranks of the group wait in its reductions
         lse = torch.full(target.shape, float("-inf"), dtype=torch.float32, device=device)
         with torch.cuda.device(device):

@@ -130,8 +130,13 @@ def test_a_group_of_one_rank():
         dist.destroy_process_group()
 
 
-def test_rows_without_a_word_need_a_group():
+@pytest.mark.parametrize("kw", [dict(vocab_start=100, vocab_size=100), dict(vocab_start=128, vocab_size=100),
+                                dict(vocab_start=50), dict(vocab_size=101), dict(vocab_start=20, vocab_size=120)])
+def test_a_part_of_the_vocabulary_needs_a_group(kw):
+    """Its loss would lack the other words, and the logits of targets among them."""
     x, w, t, _ = _case(20, 64, 100, BF16)
-    for start in (100, 128):
-        with pytest.raises(RuntimeError, match="DION_BAD_VOCAB"):
-            mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda(), vocab_start=start, vocab_size=100)
+    with pytest.raises(RuntimeError, match="DION_BAD_VOCAB"):
+        mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda(), **kw)
+    with pytest.raises(RuntimeError, match="DION_BAD_VOCAB"):
+        mda.linear_cross_entropy(x.cuda(), w.cuda(), t.cuda(), **kw)
+    mda.linear_cross_entropy_forward(x.cuda(), w.cuda(), t.cuda(), vocab_size=90)  # 10 rows of padding
