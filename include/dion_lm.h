@@ -143,6 +143,11 @@ int dion_xent_forward(const DionXentDesc* desc, const void* hidden, const void* 
  * zero grad_hidden and adds nothing to grad_weight, whatever its hidden state holds.  g is computed
  * a piece of the vocabulary at a time, in the workspace.  tokens == 0 is refused: there is no
  * gradient to add, and the caller knows it.
+ * Roundings before the products: g to bf16 (2^-8) for bf16 results, for grad_weight of up to 256 tokens
+ * to two (2^-16); where the inputs or grad_weight are fp32, g to 2^-22 of itself or 2^-49 of grad_loss_t,
+ * whichever is more, and hidden_t grad_loss_t for grad_weight to 2^-39 (bf16 inputs) or 2^-50 (fp32) of the
+ * largest of them; fp32 hidden and weight, here and in dion_xent_forward, to 2^-22 of the value or 2^-50 of
+ * the largest.
  */
 int dion_xent_backward(const DionXentDesc* desc, const void* hidden, const void* weight, const int64_t* target,
                        const float* lse, const float* grad_loss, void* grad_hidden, void* grad_weight, void* ws,

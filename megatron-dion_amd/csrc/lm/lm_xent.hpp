@@ -24,7 +24,8 @@
 // into fp16's range comes from its largest finite value; g's is known, |p - [v = y]| <= 1 times the
 // mantissa of the token's gl, whose power of two goes into X (for dW) or is put back at the end (for dX).
 // Two limbs of g are off by 2^-22 of it or by 2^-49 of |gl|, whichever is more: a word's row keeps fp32's
-// bits down to p = 1e-8 and has 9 left at 1e-12; below 1e-15 it is 0.
+// bits down to p = 1e-8 and has 9 left at 1e-12; below 1e-15 it is 0.  bf16 hidden states times that power of
+// two are one limb: off by 2^-39 of the largest of these products.
 
 namespace xent {
 

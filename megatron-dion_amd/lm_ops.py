@@ -390,11 +390,13 @@ def linear_cross_entropy_backward(grad_loss: torch.Tensor, hidden: torch.Tensor,
     `grad_weight` (fp32 or bf16, e.g. `weight.main_grad`) is written, or with `accumulate` added to, rows
     past `vocab_size` as zeros; without it a new tensor of weight's dtype is returned.  The logits'
     gradient is rounded to bf16 for the matrix cores where the result is bf16 (for grad_weight of up to 256
-    tokens, where few roundings do not average out, to two), and to two fp16 limbs where
-    it is fp32: off by 2^-22 of itself or by 2^-49 of the token's grad_loss, whichever is more (the gradient of
-    a word of probability 1e-12 has 9 bits, below 1e-15 it is 0).  fp32 hidden states and weights are two
-    such limbs: off by 2^-22 of the value or 2^-50 of the tensor's largest.  With `group`, grad_hidden is summed
-    over the vocabulary's shards."""
+    tokens, where few roundings do not average out, to two), and to two fp16 limbs where it is fp32: off by
+    2^-22 of itself or by 2^-49 of the token's grad_loss, whichever is more (the gradient of a word of
+    probability 1e-12 has 9 bits, below 1e-15 it is 0).  fp32 hidden states and weights are two such limbs: off
+    by 2^-22 of the value or 2^-50 of the tensor's largest.  For an fp32 grad_weight a token's hidden states
+    take the power of two of its grad_loss along and are off by 2^-39 (bf16) or 2^-50 (fp32) of the largest such
+    product: a token whose grad_loss is 2^-39 of the largest adds nothing.  With `group`, grad_hidden is
+    summed over the vocabulary's shards."""
     gw = _grad_weight(weight, grad_weight, accumulate, "grad_weight") if need_weight else None
     d, nbytes = _xent_desc(_lm_lib.XENT_BACKWARD, hidden, weight, target, vocab_start, vocab_size, ignore_index, gw,
                            accumulate, piece_bytes)
